@@ -21,6 +21,10 @@
  *   layers/attention.py:7-108 store_kvcache            kvx_store_kvcache,
  *                                                        kvx_store_kvcache_layers
  *
+ * Beside these stand a 4-bit form of the cache (kvx_store_kvcache_q4,
+ * kvx_load_kvcache_q4) and the attention that reads either cache
+ * (kvx_paged_attention).
+ *
  * Conventions
  *   - Every function returns an int status: KVX_OK (0) or one of the KVX_E*
  *     codes below. kvx_last_error() returns a message for the calling
@@ -70,7 +74,8 @@ extern "C" {
 #define KVX_DEV_TIMEOUT 0x08        /* a bounded wait on a peer flag ran out */
 #define KVX_DEV_COUNT_MISMATCH 0x10 /* destination posted a different block count than the source moves */
 #define KVX_DEV_PEER_FAILED 0x20    /* the peer signalled that its side of the transfer failed */
-#define KVX_DEV_PIPE_TIMEOUT 0x40   /* a bounded wait on a bulk-copy barrier ran out */
+#define KVX_DEV_PIPE_TIMEOUT 0x40   /* a bounded wait on a bulk-copy or tensor-core barrier ran out */
+#define KVX_DEV_BAD_LEN 0x80        /* a context length or cu_seqlens entry was out of range */
 
 /* ---- layout descriptor -------------------------------------------------- */
 typedef struct kvx_cache_desc {
@@ -323,6 +328,84 @@ int kvx_store_kvcache_layers(int32_t device, int32_t num_layers, const void* key
                              int64_t cache_slot_stride, const int64_t* slot_mapping_dev, int64_t num_tokens,
                              int64_t num_blocks, int32_t block_size, int64_t row_bytes, int32_t* status_dev,
                              void* stream);
+
+/* ---- 4-bit KV cache ---------------------------------------------------------
+ * A row of head_dim elements (one token, one kv head) is cut into groups of 16.
+ * A group holds one scale s = e4m3(amax / 6) and 16 codes e2m1(x / s), both
+ * rounded to the nearest, ties to even, and saturating at the largest finite
+ * value (448 and 6); x is divided by the cache's power-of-two k_scale or
+ * v_scale first. Where s rounds to 0 the codes are 0. A group with an infinity
+ * or a NaN gets the scale NaN and reads back as NaN. Two codes share a byte,
+ * the even element in the low half. A page is, kv head by kv head,
+ *   codes [block_size, head_dim / 2], then scales [block_size, head_dim / 16],
+ * so a (page, head) is one contiguous run of block_size * head_dim * 9 / 16
+ * bytes, and a page is `kv_heads` such runs in a row: to the block mover it is
+ * an opaque chunk, 3.56x smaller than a 16-bit one.
+ * head_dim must be a multiple of 16 and at most 256, block_size a multiple of
+ * 16; strides and addresses multiples of 16 bytes. dtype: 0 = bf16, 1 = fp16.
+ * Slots as in kvx_store_kvcache: -1 is padding, others outside the cache are
+ * skipped and flagged with KVX_DEV_BAD_SLOT; two tokens of one call must not
+ * share a slot. kvx_load_kvcache_q4 reads rows back (code * s * k_scale,
+ * rounded to dtype); rows of padding or bad slots are zero. */
+int kvx_store_kvcache_q4(int32_t device, int32_t dtype, const void* key_dev, const void* value_dev,
+                         int64_t key_token_stride, int64_t value_token_stride, void* k_cache_dev, void* v_cache_dev,
+                         int64_t cache_block_stride, const int64_t* slot_mapping_dev, int64_t num_tokens,
+                         int64_t num_blocks, int32_t block_size, int32_t kv_heads, int32_t head_dim, float k_scale,
+                         float v_scale, int32_t* status_dev, void* stream);
+int kvx_load_kvcache_q4(int32_t device, int32_t dtype, void* key_dev, void* value_dev, int64_t key_token_stride,
+                        int64_t value_token_stride, const void* k_cache_dev, const void* v_cache_dev,
+                        int64_t cache_block_stride, const int64_t* slot_mapping_dev, int64_t num_tokens,
+                        int64_t num_blocks, int32_t block_size, int32_t kv_heads, int32_t head_dim, float k_scale,
+                        float v_scale, int32_t* status_dev, void* stream);
+
+/* ---- attention over the paged cache -----------------------------------------
+ * Token t (of q_len) of sequence s stands at position p = context_lens[s] -
+ * q_len + t and sees the keys j <= p of that sequence with p - j < window (every
+ * one when window is 0) or j < sinks:
+ *   out = sum_j softmax_j(scale * q . k_j) * v_j,   0 when no key is visible.
+ * Query head h reads kv head h / (num_heads / num_kv_heads). Key j lies in page
+ * block_tables[s, j / block_size]. q_len is 1 without cu_seqlens_q (num_tokens ==
+ * num_seqs), else cu_seqlens_q[s + 1] - cu_seqlens_q[s]; token rows outside
+ * [cu_seqlens_q[0], cu_seqlens_q[num_seqs]) are left as they were. Scores,
+ * maxima, sums and outputs are held in fp32; the weights are rounded to the
+ * tensor cores' 16-bit type before they meet the values.
+ * A page id outside [0, num_blocks) reads as zeros and is flagged with
+ * KVX_DEV_BAD_SRC_ID; a context length outside [0, table_width * block_size] is
+ * held in it and a sequence whose cu_seqlens_q entries are out of order or range
+ * is skipped (its rows are undefined), both flagged with KVX_DEV_BAD_LEN.
+ * All device reads of lengths, tables and data follow earlier work on `stream`;
+ * nothing is read on the host, so the call can be captured and replayed with
+ * other lengths. `workspace_dev` holds partial results where the keys are split
+ * (kvx_attention_workspace bytes, 16-byte aligned; may be NULL when that is 0);
+ * calls that overlap need workspaces of their own. */
+typedef struct kvx_attention {
+    uint64_t query, out;             /* [num_tokens, num_heads, head_dim], 16-bit */
+    uint64_t k_cache, v_cache;       /* 16-bit: [N, block_size, kv_heads, head_dim]; 4-bit: pages as above */
+    uint64_t block_tables;           /* int32 [num_seqs, table_width] */
+    uint64_t context_lens;           /* int32 [num_seqs] */
+    uint64_t cu_seqlens_q;           /* int32 [num_seqs + 1], or 0: one token per sequence */
+    int64_t query_token_stride, query_head_stride; /* bytes; rows of head_dim elements are contiguous */
+    int64_t out_token_stride, out_head_stride;
+    int64_t cache_block_stride;      /* bytes, K and V alike */
+    int64_t cache_slot_stride;       /* bytes (16-bit caches) */
+    int64_t cache_head_stride;       /* bytes (16-bit caches) */
+    int64_t table_stride;            /* entries from one sequence's table row to the next */
+    int64_t num_blocks;
+    int32_t num_tokens, num_seqs, num_heads, num_kv_heads;
+    int32_t head_dim;                /* 64 or 128 */
+    int32_t block_size;
+    int32_t table_width;
+    int32_t dtype;                   /* 0 = bf16, 1 = fp16 */
+    int32_t cache_bits;              /* 16 (of dtype) or 4 */
+    int32_t window;                  /* 0: none */
+    int32_t sinks;
+    float scale;                     /* > 0 */
+    float k_scale, v_scale;          /* 4-bit caches; powers of two */
+    int32_t reserved[2];             /* must be 0 */
+} kvx_attention;
+int kvx_attention_workspace(int32_t device, const kvx_attention* args, uint64_t* bytes_out);
+int kvx_paged_attention(int32_t device, const kvx_attention* args, void* workspace_dev, uint64_t workspace_bytes,
+                        int32_t* status_dev, void* stream);
 
 /* ---- bounded waits for tests of the failure path -------------------------
  * Waits on *flag_dev >= expected with a timeout; ORs KVX_DEV_TIMEOUT into

@@ -18,8 +18,9 @@ from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
 REPO_ROOT = PKG_DIR.parent
-SOURCES = [PKG_DIR / "csrc" / "kvx.cu"]
-HEADERS = [REPO_ROOT / "include" / "kvx.h", PKG_DIR / "csrc" / "kvx_device.cuh"]
+SOURCES = [PKG_DIR / "csrc" / name for name in ("kvx.cu", "kvx_q4.cu", "kvx_attn.cu", "kvx_attn_split.cu")]
+HEADERS = [REPO_ROOT / "include" / "kvx.h"] + [
+    PKG_DIR / "csrc" / name for name in ("kvx_device.cuh", "kvx_host.h", "kvx_attn.cuh")]
 OUTPUT = PKG_DIR / "_kvx.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -33,6 +34,8 @@ NVCC_FLAGS = [
     "-cudart",
     "static",
     "--expt-relaxed-constexpr",
+    "--threads",
+    "0",
 ]
 
 

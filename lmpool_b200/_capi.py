@@ -12,6 +12,7 @@ ABI version, importing the transfer path raises.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -34,6 +35,7 @@ DEV_TIMEOUT = 0x08
 DEV_COUNT_MISMATCH = 0x10
 DEV_PEER_FAILED = 0x20
 DEV_PIPE_TIMEOUT = 0x40
+DEV_BAD_LEN = 0x80
 
 _DEV_BITS = {
     DEV_BAD_SRC_ID: "source block id out of range",
@@ -42,7 +44,8 @@ _DEV_BITS = {
     DEV_TIMEOUT: "timed out waiting for the peer",
     DEV_COUNT_MISMATCH: "peer posted a different block count",
     DEV_PEER_FAILED: "peer reported failure",
-    DEV_PIPE_TIMEOUT: "bulk-copy pipeline wait ran out",
+    DEV_PIPE_TIMEOUT: "bulk-copy or tensor-core pipeline wait ran out",
+    DEV_BAD_LEN: "context length or cu_seqlens entry out of range",
 }
 
 
@@ -120,9 +123,13 @@ class Tuning(ctypes.Structure):
     ]
 
 
+# kvx_attention, field by field (packing bytes costs less per call than filling a ctypes structure).
+pack_attention = struct.Struct("=7Q9q11i3f2i").pack
+
 _i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
 _u64 = ctypes.c_uint64
+_f32 = ctypes.c_float
 _vp = ctypes.c_void_p
 _P = ctypes.POINTER
 
@@ -167,6 +174,16 @@ SIGNATURES: dict[str, tuple] = {
         [_i32, _i32, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _i32,
          _i64, _vp, _vp],
     ),
+    "kvx_store_kvcache_q4": (
+        _i32,
+        [_i32, _i32, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i32, _i32, _i32, _f32, _f32, _vp, _vp],
+    ),
+    "kvx_load_kvcache_q4": (
+        _i32,
+        [_i32, _i32, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i32, _i32, _i32, _f32, _f32, _vp, _vp],
+    ),
+    "kvx_attention_workspace": (_i32, [_i32, ctypes.c_char_p, _P(_u64)]),
+    "kvx_paged_attention": (_i32, [_i32, ctypes.c_char_p, _vp, _u64, _vp, _vp]),
     "kvx_wait_flag": (_i32, [_i32, _vp, _u64, _u64, _vp, _vp]),
 }
 

@@ -12,8 +12,17 @@ so they can be captured in a CUDA graph (model_runner.py:630-683). Slots
 outside ``[-1, num_blocks * block_size)`` are skipped and recorded in a
 per-device status word (``kv_transfer.check_device_status``); the reference
 kernel would write out of bounds for them.
+
+Beside them stand a 4-bit form of the cache (``store_kvcache_q4``,
+``load_kvcache_q4``) and the attention that reads either cache
+(``paged_attention``, ``paged_attention_q4``): what LMPool's
+``Attention.forward`` does right after the store (attention.py:490-507), with
+an optional sliding window and sinks.
 """
 from __future__ import annotations
+
+import ctypes
+import functools
 
 import torch
 
@@ -133,3 +142,292 @@ def store_kvcache_layers(
         _status_word(device).data_ptr(), _raw_stream(device))
     if rc:
         _capi.check(rc, "kvx_store_kvcache_layers")
+
+
+# ---------------------------------------------------------------------------
+# 4-bit cache
+# ---------------------------------------------------------------------------
+
+_DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1}
+
+
+def q4_row_bytes(head_dim: int) -> int:
+    """Bytes of one token's row of one kv head in a 4-bit cache: ``head_dim / 2`` of codes and ``head_dim / 16``
+    of scales. A 4-bit cache is a ``uint8`` tensor ``[..., N, block_size, H, q4_row_bytes(D)]``; inside a page the
+    bytes are laid out head by head, codes before scales (include/kvx.h), so only whole pages are meaningful. The
+    block mover (``kv_transfer``) takes such a cache as it takes any other."""
+    if head_dim <= 0 or head_dim % 16:
+        raise ValueError(f"head_dim must be a multiple of 16, got {head_dim}")
+    return head_dim // 2 + head_dim // 16
+
+
+def _q4_check(k_cache: torch.Tensor, v_cache: torch.Tensor, block_size: int, head_dim: int) -> None:
+    if k_cache.dtype != torch.uint8 or v_cache.dtype != torch.uint8:
+        raise TypeError("a 4-bit cache holds bytes: k_cache and v_cache must be uint8")
+    if k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride():
+        raise RuntimeError("k_cache and v_cache must have the same shape and strides")
+    if k_cache.dim() != 4:
+        raise RuntimeError("k_cache must be [num_blocks, block_size, num_kv_heads, head_dim / 2 + head_dim / 16]")
+    _, bs, H, row = k_cache.shape
+    if bs != block_size or row != q4_row_bytes(head_dim):
+        raise RuntimeError(f"a 4-bit cache for block_size {block_size} and head_dim {head_dim} is [num_blocks, "
+                           f"{block_size}, num_kv_heads, {q4_row_bytes(head_dim)}], got {list(k_cache.shape)}")
+    st = k_cache.stride()
+    if st[3] != 1 or (H > 1 and st[2] != row) or (bs > 1 and st[1] != H * row):
+        raise RuntimeError("each page [block_size, num_kv_heads, row] of a 4-bit cache must be contiguous")
+
+
+def _rows_of(x: torch.Tensor) -> torch.Tensor:
+    """x [T, H, D] with contiguous, 16-byte aligned token rows (a copy where it has none)."""
+    T, H, D = x.shape
+    st = x.stride()
+    if st[2] == 1 and (H == 1 or st[1] == D) and st[0] * x.element_size() % 16 == 0 and x.data_ptr() % 16 == 0:
+        return x
+    return x.contiguous() if not x.is_contiguous() else x.clone()
+
+
+def _check_slots(slot_mapping: torch.Tensor) -> torch.Tensor:
+    if slot_mapping.dtype != torch.int64:
+        raise TypeError(f"slot_mapping must be int64, got {slot_mapping.dtype}")
+    return slot_mapping if slot_mapping.is_contiguous() else slot_mapping.contiguous()
+
+
+def store_kvcache_q4(
+    key: torch.Tensor,
+    value: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    slot_mapping: torch.Tensor,
+    block_size: int,
+    k_scale: float = 1.0,
+    v_scale: float = 1.0,
+) -> None:
+    """:func:`store_kvcache` into a 4-bit cache: rows are rounded to 4 bits on the way.
+
+    ``key``/``value``: bf16 or fp16 ``[T, H, D]``, ``D`` a multiple of 16 up to 256; caches: ``uint8`` ``[N,
+    block_size, H, q4_row_bytes(D)]``, ``block_size`` a multiple of 16. Every 16 elements of a row share an e4m3 scale
+    ``amax / 6`` and become e2m1 codes (4.5 bits an element), all rounded to the nearest, ties to even. A group with an
+    infinity or a NaN reads back as NaN. The scales reach from 2^-9 to 448 (elements up to 2688); ``k_scale`` and
+    ``v_scale``, powers of two, divide what is stored where rows lie outside that, and every reader of the cache takes
+    the same two numbers. Slots as in :func:`store_kvcache`; two tokens of a call must not share one.
+    """
+    T, H, D = key.shape
+    if value.shape != key.shape:
+        raise RuntimeError("key and value must have the same shape")
+    if key.dtype not in _DTYPE_CODE or value.dtype != key.dtype:
+        raise TypeError(f"key and value must both be bfloat16 or float16, got {key.dtype} and {value.dtype}")
+    assert slot_mapping.numel() == T, "Slot mapping size must match number of tokens"
+    _q4_check(k_cache, v_cache, block_size, D)
+    if k_cache.shape[2] != H:
+        raise RuntimeError("key/value [T, H, D] must match the cache's kv heads")
+    slot_mapping = _check_slots(slot_mapping)
+    device = _device_of(key, value, k_cache, v_cache, slot_mapping)
+    if T == 0:
+        return
+    key, value = _rows_of(key), _rows_of(value)
+    rc = _capi.lib().kvx_store_kvcache_q4(
+        device, _DTYPE_CODE[key.dtype], key.data_ptr(), value.data_ptr(), key.stride(0) * 2, value.stride(0) * 2,
+        k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), slot_mapping.data_ptr(), T, k_cache.shape[0],
+        int(block_size), H, D, k_scale, v_scale, _status_word(device).data_ptr(), _raw_stream(device))
+    if rc:
+        _capi.check(rc, "kvx_store_kvcache_q4")
+
+
+def load_kvcache_q4(
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    slot_mapping: torch.Tensor,
+    block_size: int,
+    dtype: torch.dtype = torch.bfloat16,
+    k_scale: float = 1.0,
+    v_scale: float = 1.0,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows of a 4-bit cache as ``dtype`` (bf16 or fp16) ``key, value [T, H, D]``: what :func:`store_kvcache_q4` kept
+    of them. With ``k_scale`` and ``v_scale`` of 1 every value is exact in either type. Rows of slot -1 are zero. To
+    turn pages of a 4-bit cache into pages of a 16-bit one, pass the result to :func:`store_kvcache`."""
+    if dtype not in _DTYPE_CODE:
+        raise TypeError(f"dtype must be bfloat16 or float16, got {dtype}")
+    if k_cache.dim() != 4 or k_cache.shape[3] % 9:
+        raise RuntimeError("k_cache must be [num_blocks, block_size, num_kv_heads, head_dim / 2 + head_dim / 16]")
+    D = k_cache.shape[3] // 9 * 16
+    _q4_check(k_cache, v_cache, block_size, D)
+    slot_mapping = _check_slots(slot_mapping)
+    device = _device_of(k_cache, v_cache, slot_mapping)
+    T, H = slot_mapping.numel(), k_cache.shape[2]
+    key = torch.empty((T, H, D), dtype=dtype, device=k_cache.device)
+    value = torch.empty_like(key)
+    if T == 0:
+        return key, value
+    rc = _capi.lib().kvx_load_kvcache_q4(
+        device, _DTYPE_CODE[dtype], key.data_ptr(), value.data_ptr(), H * D * 2, H * D * 2, k_cache.data_ptr(),
+        v_cache.data_ptr(), k_cache.stride(0), slot_mapping.data_ptr(), T, k_cache.shape[0], int(block_size), H, D,
+        k_scale, v_scale, _status_word(device).data_ptr(), _raw_stream(device))
+    if rc:
+        _capi.check(rc, "kvx_load_kvcache_q4")
+    return key, value
+
+
+# ---------------------------------------------------------------------------
+# Attention over the paged cache
+# ---------------------------------------------------------------------------
+
+@functools.lru_cache(maxsize=1024)
+def _attention_workspace(device: int, args: bytes) -> int:
+    out = ctypes.c_uint64(0)
+    _capi.check(_capi.lib().kvx_attention_workspace(device, args, ctypes.byref(out)), "kvx_attention_workspace")
+    return out.value
+
+
+def _paged_attention(query, k_cache, v_cache, block_tables, context_lens, block_size, cu_seqlens_q, scale, window, sinks,
+                     out, bits, k_scale, v_scale):
+    if query.dim() != 3:
+        raise RuntimeError("query must be [num_tokens, num_heads, head_dim]")
+    T, heads, D = query.shape
+    dtype = query.dtype
+    if dtype not in _DTYPE_CODE:
+        raise TypeError(f"query must be bfloat16 or float16, got {dtype}")
+    if D != 64 and D != 128:
+        raise RuntimeError(f"head_dim must be 64 or 128, got {D}")
+    if bits == 4:
+        _q4_check(k_cache, v_cache, block_size, D)
+        st = k_cache.stride()
+        block_stride, slot_stride, head_stride = st[0], 0, 0
+    else:
+        if k_cache.dtype != dtype or v_cache.dtype != dtype:
+            raise TypeError("query and cache dtypes must match")
+        if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+            raise RuntimeError("k_cache and v_cache must both be [num_blocks, block_size, num_kv_heads, head_dim]")
+        st = k_cache.stride()
+        if st != v_cache.stride():
+            raise RuntimeError("k_cache and v_cache must have the same strides")
+        if k_cache.shape[1] != block_size or k_cache.shape[3] != D:
+            raise RuntimeError(f"the cache's pages [block_size, num_kv_heads, head_dim] do not match block_size "
+                               f"{block_size} and head_dim {D}")
+        if st[3] != 1:
+            raise RuntimeError("the cache's head_dim must be contiguous")
+        block_stride, slot_stride, head_stride = 2 * st[0], 2 * st[1], 2 * st[2]
+    kv_heads = k_cache.shape[2]
+    if kv_heads == 0 or heads % kv_heads:
+        raise RuntimeError(f"{heads} query heads are no multiple of {kv_heads} kv heads")
+    if block_tables.dtype != torch.int32 or context_lens.dtype != torch.int32:
+        raise TypeError("block_tables and context_lens must be int32")
+    if block_tables.dim() != 2 or context_lens.dim() != 1 or block_tables.shape[0] != context_lens.shape[0]:
+        raise RuntimeError("block_tables must be [num_seqs, width] and context_lens [num_seqs]")
+    S, width = block_tables.shape
+    if width > 1 and block_tables.stride(1) != 1:
+        block_tables = block_tables.contiguous()
+    if S > 1 and context_lens.stride(0) != 1:
+        context_lens = context_lens.contiguous()
+    cu = 0
+    if cu_seqlens_q is None:
+        if T != S:
+            raise RuntimeError(f"without cu_seqlens_q every sequence has one token: {T} tokens, {S} sequences")
+        device = _device_of(query, k_cache, v_cache, block_tables, context_lens)
+    else:
+        if cu_seqlens_q.dtype != torch.int32:
+            raise TypeError(f"cu_seqlens_q must be int32, got {cu_seqlens_q.dtype}")
+        if cu_seqlens_q.dim() != 1 or cu_seqlens_q.shape[0] != S + 1:
+            raise RuntimeError(f"cu_seqlens_q must hold num_seqs + 1 = {S + 1} entries")
+        if S > 0 and cu_seqlens_q.stride(0) != 1:
+            cu_seqlens_q = cu_seqlens_q.contiguous()
+        device = _device_of(query, k_cache, v_cache, block_tables, context_lens, cu_seqlens_q)
+        cu = cu_seqlens_q.data_ptr()
+    if window is not None and window <= 0:
+        raise ValueError(f"window must be positive (None: every key), got {window}")
+    if sinks < 0:
+        raise ValueError(f"sinks must not be negative, got {sinks}")
+    # Positions are 32-bit: a window or sinks beyond them are all the same.
+    window = 0 if window is None else min(int(window), 2 ** 31 - 1)
+    sinks = min(int(sinks), 2 ** 31 - 1)
+    qs = query.stride()
+    if qs[2] != 1 or qs[0] % 8 or qs[1] % 8 or query.data_ptr() % 16:
+        query = query.contiguous() if not query.is_contiguous() else query.clone()
+        qs = query.stride()
+    if out is None:
+        out = torch.empty((T, heads, D), dtype=dtype, device=query.device)
+    else:
+        if out.shape != query.shape or out.dtype != dtype:
+            raise RuntimeError("out must have query's shape and dtype")
+        _device_of(query, out)
+        os = out.stride()
+        if os[2] != 1 or os[0] % 8 or os[1] % 8 or out.data_ptr() % 16:
+            raise RuntimeError("out must have contiguous, 16-byte aligned rows of head_dim")
+    os = out.stride()
+    if T == 0 or S == 0:
+        return out
+    sizes = (T, S, heads, kv_heads, D, block_size, width, _DTYPE_CODE[dtype], bits, window, sinks,
+             D ** -0.5 if scale is None else float(scale), k_scale, v_scale, 0, 0)
+    pointers = (query.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(),
+                context_lens.data_ptr(), cu, 2 * qs[0], 2 * qs[1], 2 * os[0], 2 * os[1], block_stride, slot_stride,
+                head_stride, block_tables.stride(0), k_cache.shape[0])
+    # Sizes alone decide how much workspace a call needs.
+    need = _attention_workspace(device, _capi.pack_attention(*_NO_POINTERS[cu != 0], *sizes))
+    workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
+    rc = _capi.lib().kvx_paged_attention(
+        device, _capi.pack_attention(*pointers, *sizes), workspace.data_ptr() if need else None, need,
+        _status_word(device).data_ptr(), _raw_stream(device))
+    if rc:
+        _capi.check(rc, "kvx_paged_attention")
+    return out
+
+
+_NO_POINTERS = {False: (0,) * 15 + (1,), True: (0,) * 6 + (1,) + (0,) * 8 + (1,)}
+
+
+def paged_attention(
+    query: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    block_size: int,
+    *,
+    cu_seqlens_q: torch.Tensor | None = None,
+    scale: float | None = None,
+    window: int | None = None,
+    sinks: int = 0,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Causal attention of new tokens over the paged cache they were stored in, optionally with a sliding window and
+    a few first tokens that stay visible (sinks).
+
+    ``query``: bf16 or fp16 ``[T, Hq, D]``, ``D`` 64 or 128; caches ``[N, block_size, H, D]`` of the same type, as
+    :func:`store_kvcache` fills them (any strides over blocks, slots and heads that are multiples of 16 bytes);
+    ``block_tables`` int32 ``[S, width]`` page ids; ``context_lens`` int32 ``[S]``: tokens of each sequence in the
+    cache, the new ones among them. Query head ``h`` reads kv head ``h // (Hq // H)``.
+
+    Without ``cu_seqlens_q`` each sequence has one new token (``T == S``, decode). With it (int32 ``[S + 1]``, rising
+    from 0) sequence ``s`` has the tokens ``cu_seqlens_q[s]`` to ``cu_seqlens_q[s + 1]``, the last of its context:
+    prompts, chunks of prompts, drafted tokens. Token at position ``p`` sees key ``j <= p`` if ``window`` is None, if
+    ``p - j < window`` or if ``j < sinks``. A token that sees no key gets zeros. Rows behind the last sequence are left
+    as they were. ``scale`` (default ``D ** -0.5``) must be positive.
+
+    Runs on the current stream without synchronising; lengths and tables are read on the device, so a captured call
+    can be replayed with others. Bad page ids (their keys read as zeros) and lengths are recorded in the device's
+    status word (``kv_transfer.check_device_status``).
+    """
+    return _paged_attention(query, k_cache, v_cache, block_tables, context_lens, block_size, cu_seqlens_q, scale, window,
+                            sinks, out, 16, 1.0, 1.0)
+
+
+def paged_attention_q4(
+    query: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    block_size: int,
+    *,
+    cu_seqlens_q: torch.Tensor | None = None,
+    scale: float | None = None,
+    window: int | None = None,
+    sinks: int = 0,
+    k_scale: float = 1.0,
+    v_scale: float = 1.0,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """:func:`paged_attention` over a 4-bit cache (``uint8`` ``[N, block_size, H, q4_row_bytes(D)]``, filled by
+    :func:`store_kvcache_q4` with the same ``k_scale`` and ``v_scale``). The cache is read as 4.5 bits an element and
+    widened, exactly, next to the products."""
+    return _paged_attention(query, k_cache, v_cache, block_tables, context_lens, block_size, cu_seqlens_q, scale, window,
+                            sinks, out, 4, k_scale, v_scale)

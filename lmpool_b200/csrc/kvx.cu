@@ -37,6 +37,7 @@
 
 #include "kvx.h"
 #include "kvx_device.cuh"
+#include "kvx_host.h"
 
 namespace kvx {
 
@@ -44,7 +45,6 @@ constexpr int kMaxSegments = 8;
 constexpr int kRegThreads = 256;
 constexpr int kRegUnroll = 4;
 constexpr int kStoreThreads = 64;   // one token's K row and V row per CTA
-constexpr int kMaxDevices = 64;
 constexpr uint64_t kFailBit = 1ull << 63;
 // Upper bound on mbarrier polls of a bulk-copy stage before the pipeline
 // gives up (each poll may suspend for a hardware-chosen interval).
@@ -541,32 +541,6 @@ int fail(int code, const char* fmt, ...) {
 int cuda_fail(cudaError_t e, const char* what) {
     return fail(KVX_ECUDA, "%s: %s (%s)", what, cudaGetErrorName(e), cudaGetErrorString(e));
 }
-
-#define KVX_CUDA(call, what)                         \
-    do {                                             \
-        cudaError_t e_ = (call);                     \
-        if (e_ != cudaSuccess) return cuda_fail(e_, what); \
-    } while (0)
-
-struct DeviceGuard {
-    int prev = -1;
-    bool changed = false;
-    cudaError_t err = cudaSuccess;
-    explicit DeviceGuard(int dev) {
-        err = cudaGetDevice(&prev);
-        if (err == cudaSuccess && prev != dev) {
-            err = cudaSetDevice(dev);
-            changed = (err == cudaSuccess);
-        }
-    }
-    ~DeviceGuard() {
-        if (changed) cudaSetDevice(prev);
-    }
-};
-
-#define KVX_DEVICE_GUARD(dev)                                            \
-    DeviceGuard guard_(dev);                                             \
-    if (guard_.err != cudaSuccess) return cuda_fail(guard_.err, "select device")
 
 std::mutex g_mu;
 kvx_tuning g_tuning = {0, 0, 0, 0, 0, 0};

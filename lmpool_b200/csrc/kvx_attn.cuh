@@ -1,0 +1,282 @@
+// Shared by the paged-attention kernels: launch parameters, the cut of a call
+// into work items, the keys an item reads, tensor-core and 4-bit helpers.
+//
+// Row r of an item is query head (r % G) of its kv head's group and token
+// (r / G) of its run of tokens, so that all rows of an item share one kv head
+// and every key is read once for G heads. Token t of sequence s stands at
+// position p = context_len - q_len + t and sees key j when
+//     j <= p  and  (p - j < window  or  j < sinks).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+#include "kvx.h"
+#include "kvx_device.cuh"
+
+namespace kvx {
+
+struct AttnParams {
+    const char* q;
+    char* out;
+    const char* k;
+    const char* v;
+    int64_t q_token_stride, q_head_stride;    // bytes
+    int64_t o_token_stride, o_head_stride;
+    int64_t block_stride, slot_stride, head_stride;
+    int64_t num_blocks;
+    const int32_t* table;
+    int64_t table_stride;                     // entries
+    const int32_t* ctx;
+    const int32_t* cu;                        // nullptr: one token per sequence
+    int32_t* status;
+    float* ws_o;                              // [tokens * heads][splits][D], not yet divided by the sum
+    float* ws_ml;                             // [tokens * heads][splits][2]: maximum of scale_log2 * score, sum
+    float scale_log2;                         // scale * log2(e) (* k_scale of a 4-bit cache)
+    float out_scale;                          // v_scale of a 4-bit cache, else 1
+    int32_t table_width, block_size, block_shift;   // block_shift < 0: not a power of two
+    int32_t num_seqs, num_tokens;
+    int32_t heads, kv_heads, group;
+    int32_t window, sinks;                    // window: INT_MAX when there is none
+    int32_t splits;
+    int32_t tile_tokens;                      // tokens of an item
+    int32_t tile_slots;                       // item slots per (kv head, split)
+};
+
+struct AttnItem {
+    int seq;
+    int q0;        // first token row
+    int tokens;    // tokens of this item (0: nothing to do)
+    int pos0;      // position of the first token (negative: before the context)
+    int head;      // kv head
+    int split;
+};
+
+// Length of sequence s's context, held in what its table can address.
+__device__ __forceinline__ int context_of(const AttnParams& p, int s) {
+    const int64_t cap = static_cast<int64_t>(p.table_width) * p.block_size;
+    int64_t c = p.ctx[s];
+    if (c < 0 || c > cap) {
+        atomicOr(p.status, KVX_DEV_BAD_LEN);
+        c = c < 0 ? 0 : cap;
+    }
+    return static_cast<int>(c);
+}
+
+// Tile slot `x` of a call. Without cu_seqlens a slot is a sequence. With them
+// the slots of sequence s start at cu[s] / tile + s: that leaves every
+// sequence at least ceil(len / tile) of them, needs no prefix sum and no
+// host copy of the lengths; spare slots hold no tokens.
+__device__ __forceinline__ AttnItem locate_item(const AttnParams& p, int x) {
+    AttnItem it;
+    it.tokens = 0;
+    it.head = 0;
+    it.split = 0;
+    if (p.cu == nullptr) {
+        it.seq = x;
+        it.q0 = x;
+        it.tokens = 1;
+        it.pos0 = context_of(p, x) - 1;
+        return it;
+    }
+    int lo = 0, hi = p.num_seqs - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (p.cu[mid] / p.tile_tokens + mid <= x) lo = mid;
+        else hi = mid - 1;
+    }
+    it.seq = lo;
+    const int a = p.cu[lo], b = p.cu[lo + 1];
+    if (a < 0 || b < a || b > p.num_tokens) {
+        atomicOr(p.status, KVX_DEV_BAD_LEN);
+        it.q0 = it.pos0 = 0;
+        return it;
+    }
+    const int64_t first = static_cast<int64_t>(x - (a / p.tile_tokens + lo)) * p.tile_tokens;
+    it.q0 = static_cast<int>(a + (first < 0 ? 0 : first));
+    it.pos0 = 0;
+    if (first < 0 || first >= b - a) return it;
+    it.tokens = static_cast<int>(b - a - first < p.tile_tokens ? b - a - first : p.tile_tokens);
+    it.pos0 = static_cast<int>(context_of(p, lo) - (b - a) + first);
+    return it;
+}
+
+// Keys of an item in tiles of KT: the tiles that hold a sink, then those from
+// the oldest key of the first token's window to the last token's own key.
+struct KeyTiles {
+    int head;      // leading tiles (sinks)
+    int skip;      // tiles between them and the window
+    int begin, end;   // this split's range of tile numbers
+    template <int KT>
+    __device__ __forceinline__ int first_key(int i) const {
+        return (i < head ? i : i + skip) * KT;
+    }
+};
+
+template <int KT>
+__device__ __forceinline__ KeyTiles key_tiles(const AttnParams& p, const AttnItem& it) {
+    KeyTiles t;
+    const int last = it.pos0 + it.tokens - 1;      // newest visible key
+    t.head = t.skip = t.begin = t.end = 0;
+    if (it.tokens == 0 || last < 0) return t;
+    const int total = last / KT + 1;
+    // A first token that stands before the context sees nothing: the window that counts is the one
+    // of the first token with a position.
+    const int first = it.pos0 < 0 ? 0 : it.pos0;
+    const int lo = first >= p.window ? first - p.window + 1 : 0;
+    const int low_tile = lo / KT;
+    const int sink_tiles = p.sinks > 0 ? (min(p.sinks, last + 1) - 1) / KT + 1 : 0;
+    t.head = min(sink_tiles, low_tile);
+    t.skip = low_tile - t.head;
+    const int n = total - t.skip;
+    const int per = (n + p.splits - 1) / p.splits;
+    t.begin = min(n, it.split * per);
+    t.end = min(n, t.begin + per);
+    return t;
+}
+
+// Whether key j is visible to a token at position pos.
+__device__ __forceinline__ bool visible(const AttnParams& p, int pos, int j) {
+    return j <= pos && (pos - j < p.window || j < p.sinks);
+}
+
+// Byte offset of page `blk` of a sequence in the cache, or -1 (flagged).
+__device__ __forceinline__ int64_t page_offset(const AttnParams& p, const int32_t* table, int blk) {
+    const int64_t id = blk < p.table_width ? table[blk] : -1;
+    if (id < 0 || id >= p.num_blocks) {
+        atomicOr(p.status, KVX_DEV_BAD_SRC_ID);
+        return -1;
+    }
+    return id * p.block_stride;
+}
+
+__device__ __forceinline__ int block_of(const AttnParams& p, int j) {
+    return p.block_shift >= 0 ? j >> p.block_shift : j / p.block_size;
+}
+
+// ---------------------------------------------------------------------------
+// Numbers
+// ---------------------------------------------------------------------------
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <typename T>
+struct Pair;
+template <>
+struct Pair<__nv_bfloat16> {
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        uint32_t r;
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t x) {
+        return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+    }
+};
+template <>
+struct Pair<__half> {
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        uint32_t r;
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t x) {
+        __half2 h;
+        memcpy(&h, &x, 4);
+        return __half22float2(h);
+    }
+};
+
+// Four codes pairs (8 codes, low half of a byte first) as f16x2; the levels
+// 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives are exact in fp16.
+__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t out[4]) {
+    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+        "mov.b32 {a, b, c, d}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+        : "=r"(out[0]), "=r"(out[1]), "=r"(out[2]), "=r"(out[3])
+        : "r"(w));
+}
+// Two e4m3 scales (exact in fp16).
+__device__ __forceinline__ uint32_t scales_to_half(uint32_t two) {
+    uint32_t r;
+    const uint16_t v = static_cast<uint16_t>(two);
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
+    return r;
+}
+// code * scale has at most six significant bits and lies in [2^-10, 2688]: exact.
+__device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+// One element of the cache as fp32 (the rare path below).
+template <typename T, int D, bool Q4>
+__device__ __forceinline__ float cache_element(const AttnParams& p, const char* plane, int64_t page, int off, int head,
+                                               int d) {
+    const char* base = plane + page + head * p.head_stride;
+    if constexpr (Q4) {
+        const uint8_t* b = reinterpret_cast<const uint8_t*>(base);
+        const uint32_t byte = b[off * (D / 2) + d / 2];
+        const uint32_t scale = b[p.block_size * (D / 2) + off * (D / 16) + d / 16];
+        const uint32_t c = d & 1 ? byte >> 4 : byte & 15;
+        const uint32_t e = (c >> 1) & 3;
+        const float level = e ? static_cast<float>((2 + (c & 1)) << e) * 0.25f : 0.5f * (c & 1);
+        return (c & 8 ? -level : level) * Pair<__half>::unpack(scales_to_half(scale)).x;
+    } else {
+        return static_cast<float>(reinterpret_cast<const T*>(base + off * p.slot_stride)[d]);
+    }
+}
+
+// A product with a masked key is skipped in the formula, but a tile multiplies
+// every row with every key: weight 0 times a value that is infinite or NaN gives
+// NaN in rows that do not see that key. Such a row (finite sum, NaN in the
+// output) is computed again from its visible keys alone: out[d0 + i], i < N, for
+// the maximum m2 (of scale_log2 * score) that the tiles found. Only inputs that are not finite come here.
+template <typename T, int D, bool Q4, int N>
+__device__ __noinline__ void visible_keys_only(const AttnParams& p, const AttnItem& it, const KeyTiles& kt, int tile_keys,
+                                               int row, float m2, int d0, float* acc) {
+    const int token = row / p.group;
+    const int head = it.head * p.group + row % p.group;
+    const int pos = it.pos0 + token;
+    const T* q = reinterpret_cast<const T*>(p.q + (it.q0 + token) * p.q_token_stride + head * p.q_head_stride);
+    const int32_t* table = p.table + it.seq * p.table_stride;
+    for (int i = 0; i < N; ++i) acc[i] = 0.f;
+    for (int i = kt.begin; i < kt.end; ++i) {
+        const int first = (i < kt.head ? i : i + kt.skip) * tile_keys;
+        for (int j = first; j < first + tile_keys; ++j) {
+            if (!visible(p, pos, j)) continue;
+            const int blk = j / p.block_size, off = j - blk * p.block_size;
+            const int64_t page = page_offset(p, table, blk);
+            if (page < 0) continue;
+            float s = 0.f;
+            for (int d = 0; d < D; ++d)
+                s = fmaf(static_cast<float>(q[d]), cache_element<T, D, Q4>(p, p.k, page, off, it.head, d), s);
+            const float w = exp2f(fmaf(s, p.scale_log2, -m2));
+            for (int d = 0; d < N; ++d)
+                acc[d] = fmaf(w, cache_element<T, D, Q4>(p, p.v, page, off, it.head, d0 + d), acc[d]);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Launches (one translation unit per kernel family)
+// ---------------------------------------------------------------------------
+
+// Rows are few: keys split over CTAs and warps (kvx_attn_split.cu). An item has 8 * nt rows (nt = 1, 2, 4).
+int launch_attn_split(const AttnParams& p, int head_dim, int dtype, bool q4, int nt, int device, cudaStream_t stream);
+// Rows are many: 256-row tiles on the tensor cores (kvx_attn_tile.cu).
+int launch_attn_tile(const AttnParams& p, int head_dim, int dtype, bool q4, int device, int sms, cudaStream_t stream);
+// Joins the splits of either (kvx_attn_split.cu).
+int launch_attn_join(const AttnParams& p, int head_dim, int dtype, cudaStream_t stream);
+
+}  // namespace kvx

@@ -1,0 +1,101 @@
+"""CPU tests of the 4-bit cache's definition and of the refusals that need no GPU."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from lmpool_b200 import _capi
+from lmpool_b200 import attention as at
+from oracle import attention_ref as ref
+
+
+def test_row_bytes():
+    assert at.q4_row_bytes(128) == 72 and at.q4_row_bytes(64) == 36
+    with pytest.raises(ValueError):
+        at.q4_row_bytes(24)
+
+
+def test_e4m3_table_is_torchs():
+    want = torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).double().tolist()
+    assert ref.E4M3 == want
+
+
+def test_definition_keeps_values_on_the_grid():
+    """What the format can hold is kept as it is; everything else moves by at most half a step of the group."""
+    row = torch.tensor(ref.LEVELS + [-v for v in ref.LEVELS]) * 0.375
+    codes, scales = ref.q4_encode_row(row)
+    assert ref.q4_decode(codes, scales) == row.tolist()
+    x = torch.randn(4096, generator=torch.Generator().manual_seed(1))
+    back = torch.tensor(ref.q4_decode(*ref.q4_encode_row(x)), dtype=torch.float64)
+    top = x.double().view(-1, 16).abs().amax(1, keepdim=True)
+    # widest step 2 of 6 levels: half of it is top / 6, and the scale is off by at most 2^-4 (e4m3)
+    assert ((back - x.double()).view(-1, 16).abs() <= top / 6 * (1 + 2.0 ** -4) + 1e-9).all()
+
+
+def test_definition_of_odd_groups():
+    assert ref.q4_encode_row(torch.zeros(16)) == ([0] * 16, [0])
+    assert ref.q4_encode_row(torch.full((16,), math.inf)) == ([0] * 16, [0x7F])
+    assert ref.q4_encode_row(torch.full((16,), 1e9))[1] == [126]
+    codes, scales = ref.q4_encode_row(torch.full((16,), 2.0 ** -10))
+    assert scales == [0] and codes == [0] * 16
+
+
+def _args(**kw):
+    base = dict(ptr=[1 << 20] * 6, cu=0, strides=[1024, 256, 1024, 256, 4096, 256, 128, 8], num_blocks=4, T=2, S=2, heads=4,
+                kv=2, dim=64, bs=16, width=8, dtype=0, bits=16, window=0, sinks=0, scale=0.1, ks=1.0, vs=1.0, r=0)
+    base.update(kw)
+    b = base
+    return _capi.pack_attention(*b["ptr"], b["cu"], *b["strides"], b["num_blocks"], b["T"], b["S"], b["heads"], b["kv"],
+                                b["dim"], b["bs"], b["width"], b["dtype"], b["bits"], b["window"], b["sinks"], b["scale"],
+                                b["ks"], b["vs"], b["r"], 0)
+
+
+BAD = [dict(r=1), dict(dtype=2), dict(bits=8), dict(dim=96), dict(T=-1), dict(S=-1), dict(heads=5), dict(kv=0),
+       dict(heads=1024, kv=2), dict(bs=0), dict(bs=8, bits=4), dict(width=-1), dict(width=1 << 28), dict(num_blocks=0),
+       dict(window=-1), dict(sinks=-1), dict(scale=0.0), dict(scale=math.nan), dict(scale=math.inf), dict(scale=-1.0),
+       dict(bits=4, ks=3.0), dict(bits=4, vs=0.0), dict(ks=2.0), dict(T=3), dict(bits=4, ks=-2.0),
+       dict(bits=4, scale=1e30, ks=2.0 ** 60), dict(bits=4, scale=1e-30, ks=2.0 ** -60)]
+BAD_POINTERS = [dict(ptr=[0] + [1 << 20] * 5), dict(ptr=[1 << 20] * 5 + [0]), dict(ptr=[8] + [1 << 20] * 5),
+                dict(strides=[1000, 256, 1024, 256, 4096, 256, 128, 8]), dict(strides=[1024, 256, 1024, 256, 4096, 250, 128, 8])]
+
+
+@pytest.mark.parametrize("bad", BAD + BAD_POINTERS, ids=str)
+def test_attention_refuses_before_touching_a_gpu(kvx_lib, bad):
+    status = ctypes.c_int32(0)
+    rc = kvx_lib.kvx_paged_attention(0, _args(**bad), None, 0, ctypes.addressof(status), None)
+    assert rc == _capi.KVX_EINVAL and kvx_lib.kvx_last_error()
+
+
+def test_attention_needs_a_status_word(kvx_lib):
+    assert kvx_lib.kvx_paged_attention(0, _args(), None, 0, None, None) == _capi.KVX_EINVAL
+    assert kvx_lib.kvx_paged_attention(0, None, None, 0, None, None) == _capi.KVX_EINVAL
+
+
+def test_attention_with_no_tokens_is_no_work(kvx_lib):
+    status = ctypes.c_int32(0)
+    assert kvx_lib.kvx_paged_attention(0, _args(T=0, S=0), None, 0, ctypes.addressof(status), None) == _capi.KVX_OK
+
+
+@pytest.mark.parametrize("bad", [dict(dtype=2), dict(T=-1), dict(N=0), dict(bs=8), dict(dim=24), dict(dim=272), dict(heads=0),
+                                 dict(ks=1.5), dict(vs=math.inf), dict(stride=1000), dict(ptr=8), dict(ptr=0)], ids=str)
+@pytest.mark.parametrize("name", ["kvx_store_kvcache_q4", "kvx_load_kvcache_q4"])
+def test_q4_rows_refuse_before_touching_a_gpu(kvx_lib, name, bad):
+    a = dict(dtype=0, T=2, N=4, bs=16, dim=64, heads=2, ks=1.0, vs=1.0, stride=256, ptr=1 << 20)
+    a.update(bad)
+    status = ctypes.c_int32(0)
+    rc = getattr(kvx_lib, name)(0, a["dtype"], a["ptr"], 1 << 20, a["stride"], 256, 1 << 20, 1 << 20, 4608, 1 << 20, a["T"],
+                                a["N"], a["bs"], a["heads"], a["dim"], a["ks"], a["vs"], ctypes.addressof(status), None)
+    assert rc == _capi.KVX_EINVAL and kvx_lib.kvx_last_error()
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros(2, 1, 64, dtype=torch.float16)
+    kc = torch.zeros(1, 16, 1, 36, dtype=torch.uint8)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        at.store_kvcache_q4(x, x, kc, kc, torch.zeros(2, dtype=torch.int64), 16)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        at.load_kvcache_q4(kc, kc, torch.zeros(2, dtype=torch.int64), 16)
+    kv = torch.zeros(1, 16, 1, 64, dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        at.paged_attention(x, kv, kv, torch.zeros(2, 1, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), 16)
