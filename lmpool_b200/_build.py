@@ -18,7 +18,7 @@ from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
 REPO_ROOT = PKG_DIR.parent
-SOURCES = [PKG_DIR / "csrc" / name for name in ("kvx.cu", "kvx_q4.cu", "kvx_attn.cu", "kvx_attn_split.cu")]
+SOURCES = [PKG_DIR / "csrc" / name for name in ("kvx.cu", "kvx_q4.cu", "kvx_attn.cu", "kvx_attn_split.cu", "kvx_attn_tile.cu")]
 HEADERS = [REPO_ROOT / "include" / "kvx.h"] + [
     PKG_DIR / "csrc" / name for name in ("kvx_device.cuh", "kvx_host.h", "kvx_attn.cuh")]
 OUTPUT = PKG_DIR / "_kvx.so"

@@ -13,7 +13,7 @@ namespace kvx {
 
 constexpr int kMaxSplits = 64;
 constexpr int kFewRows = 32;            // rows of an item of the split kernel, at most
-constexpr int kTileRows = 32;          // rows of an item of the tile kernel
+constexpr int kTileRows = 256;          // rows of an item of the tile kernel
 
 struct AttnPlan {
     bool tile;          // tile kernel, else split kernel
@@ -70,7 +70,7 @@ static AttnPlan plan_of(const kvx_attention* a, int sms) {
     const int group = a->num_heads / a->num_kv_heads;
     const int64_t tokens = a->num_tokens, seqs = std::max(1, a->num_seqs);
     const int64_t avg = (tokens + seqs - 1) / seqs;
-    pl.tile = false;
+    pl.tile = avg * group > kFewRows;
     int keys_per_tile, fill, min_tiles;
     if (pl.tile) {
         pl.tile_tokens = kTileRows / group;
@@ -181,7 +181,8 @@ int kvx_paged_attention(int32_t device, const kvx_attention* args, void* workspa
     KVX_DEVICE_GUARD(device);
     const auto st = static_cast<cudaStream_t>(stream);
     const bool q4 = a.cache_bits == 4;
-    rc = launch_attn_split(p, a.head_dim, a.dtype, q4, pl.nt, device, st);
+    rc = pl.tile ? launch_attn_tile(p, a.head_dim, a.dtype, q4, device, sms, st)
+                 : launch_attn_split(p, a.head_dim, a.dtype, q4, pl.nt, device, st);
     if (rc == KVX_OK && pl.splits > 1) rc = launch_attn_join(p, a.head_dim, a.dtype, st);
     if (rc != KVX_OK) cudaGetLastError();
     return rc;

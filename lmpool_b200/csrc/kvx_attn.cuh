@@ -219,6 +219,14 @@ __device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
     return r;
 }
 
+// What a row of bf16 queries is divided by on its way to fp16: the power of two below
+// its largest element, which keeps every element within 2^-25 of that one; 1 for
+// rows that are zero, below 2^-100 or not finite.
+__device__ __forceinline__ float row_divisor(float amax) {
+    const uint32_t e = __float_as_uint(amax) & 0x7f800000u;
+    return e < 0x0d800000u || e == 0x7f800000u ? 1.f : __uint_as_float(e);
+}
+
 // One element of the cache as fp32 (the rare path below).
 template <typename T, int D, bool Q4>
 __device__ __forceinline__ float cache_element(const AttnParams& p, const char* plane, int64_t page, int off, int head,

@@ -149,11 +149,8 @@ __global__ void __launch_bounds__(kSplitWarps * 32) attn_split_kernel(const __gr
                 }
                 amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 1));
                 amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
-                // The power of two of amax, as its exponent bits; rows that are zero, tiny or not finite keep their size.
-                uint32_t e = __float_as_uint(amax) & 0x7f800000u;
-                if (e < 0x0d800000u || e == 0x7f800000u) e = 0x3f800000u;      // below 2^-100
-                factor = __uint_as_float(e);
-                const float inv = __uint_as_float(0x7f000000u - e);
+                factor = row_divisor(amax);
+                const float inv = 1.f / factor;
 #pragma unroll
                 for (int i = 0; i < KS; ++i) {
                     const float2 a = Pair<T>::unpack(raw[i].x), b = Pair<T>::unpack(raw[i].y);

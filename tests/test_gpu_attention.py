@@ -248,6 +248,13 @@ def test_prompts(require_gpu, dtype, q4, heads, kv_heads, dim, window, sinks):
     case.check(window=window, sinks=sinks)
 
 
+@pytest.mark.parametrize("heads,kv_heads", [(48, 1), (71, 1), (256, 1)])
+@pytest.mark.parametrize("q_lens", [None, [3, 1]])
+def test_many_query_heads_on_one_kv_head(require_gpu, heads, kv_heads, q_lens):
+    case = Case([33, 200], heads, kv_heads, 128, 16, torch.bfloat16, False, q_lens=q_lens, seed=heads)
+    case.check()
+
+
 @pytest.mark.parametrize("dtype,q4", TYPES, ids=IDS)
 def test_a_chunk_on_a_long_context(require_gpu, dtype, q4):
     case = Case([1500], 4, 1, 128, 64, dtype, q4, q_lens=[70], seed=5)
