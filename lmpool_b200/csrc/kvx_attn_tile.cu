@@ -6,8 +6,9 @@
 // kv head as two 128-row tiles, so that a key tile (128 keys) read once serves both and
 // one tile's softmax runs under the other's products. Warps:
 //   0-3, 4-7  softmax of row tile 0 and 1: a thread owns a row;
-//   8-11      load queries, keys and values into shared memory;
-//   12        one thread issues the products (13-15 idle).
+//   8-11      queries into shared memory; edge tiles of a 16-bit cache; widening of a 4-bit one;
+//   12        one thread issues the products;
+//   13        issues the bulk copies (14, 15 idle).
 // Tensor memory (512 columns): S0, S1 (128 fp32 columns each), O0, O1 (D each).
 // The weights P overwrite the first half of their S as 16-bit pairs and are the A
 // operand of O += P V straight from tensor memory. Per row tile i and key tile j the
@@ -20,15 +21,27 @@
 // Shared memory holds operand rows of 64 elements (128 bytes) in the 128-byte
 // swizzle: 16-byte chunk c of row r at chunk c ^ (r % 8). Queries and keys are K-major
 // operands; values, stored key by key as they lie in the cache, are an MN-major B.
-// The loaders write them with 16-byte cp.async, so any page size and any strides work;
-// a 4-bit cache is widened to fp16 by the loaders (queries go to fp16 too, each
-// row divided by a power of two), and the products see one type.
+// A 16-bit cache whose page size is a multiple of 8 is read by TMA, one box per page (or 128 rows
+// of it) and 64 elements. The value tile that reaches behind the context, and every tile of a
+// cache of other page sizes, is gathered by 16-byte cp.async instead, with zeros for
+// keys that no row sees: what lies behind a context may be NaN, and 0 * NaN is not 0.
+// A 4-bit cache comes as raw pages through a ring of its own (bulk copies of 16 keys or more) and
+// is widened to fp16 in shared memory (queries go to fp16 too, each row divided by a power of
+// two), so that the products see one type.
+//
+// Exponentials: the special-function unit gives 16 a clock and SM, which alone is as
+// long as the products of a tile. So 3 of 8 are computed as 2^n p(f), x = n + f, |f| <=
+// 1/2, on the FMA units, with a degree-4 polynomial (relative error 2.8e-6, from a
+// weighted least-squares fit of 2^f; the weights are rounded to 2^-8 or 2^-11).
 //
 // Every wait is bounded: where one runs out, the CTA flags KVX_DEV_PIPE_TIMEOUT,
 // all warps leave their loops, and tensor memory is freed.
 
+#include <cuda.h>
+
 #include <atomic>
 #include <climits>
+#include <cmath>
 #include <type_traits>
 
 #include "kvx.h"
@@ -40,19 +53,29 @@ namespace kvx {
 constexpr int kTileThreads = 512;
 constexpr int kTileKeys = 128;
 constexpr int kHalfRows = 128;                 // rows of one of the two row tiles
+constexpr int kFmaPairs = 3;                   // of 8 pairs of exponentials, on the FMA units
 constexpr uint32_t kMaxWaitPolls = 1u << 22;   // each poll may suspend for a hardware-chosen time
-constexpr int kLag = 2;                        // loads in flight before the oldest is awaited
 
-template <int D>
+template <int D, bool Q4>
 struct TileConfig {
     static constexpr int kSlabs = D / 64;
     static constexpr int kSlabBytes = 128 * 128;                  // 128 rows of 64 elements
     static constexpr int kTileBytes = kSlabs * kSlabBytes;        // 128 rows of D elements
-    static constexpr int kStages = D == 128 ? 5 : 8;              // ring of key and value tiles
+    static constexpr int kStages = D == 128 ? (Q4 ? 4 : 5) : 8;   // ring of key and value tiles
+    static constexpr int kRawStages = Q4 ? 3 : 0;                 // ring of raw 4-bit tiles
+    static constexpr int kRawCodes = kTileKeys * D / 2;
+    static constexpr int kRawBytes = kRawCodes + kTileKeys * D / 16;
     static constexpr int kRing = 2 * kTileBytes;                  // after the two query tiles
-    static constexpr int kFactors = kRing + kStages * kTileBytes;
+    static constexpr int kRaw = kRing + kStages * kTileBytes;
+    static constexpr int kFactors = kRaw + kRawStages * kRawBytes;
     static constexpr int kBars = kFactors + 2 * kHalfRows * 4;
-    static constexpr int kSmem = 1024 + kBars + 256;
+    static constexpr int kSmem = 1024 + kBars + 512;
+};
+
+// TMA views of a 16-bit cache: [D, block_size, kv_heads, num_blocks] from the innermost.
+struct TileMaps {
+    CUtensorMap k, v;
+    int32_t box_rows;      // rows of a box; 0: no TMA
 };
 
 // ---- tcgen05 ----------------------------------------------------------------
@@ -149,6 +172,65 @@ __device__ __forceinline__ void st_shared16(uint32_t dst, uint32_t a, uint32_t b
 }
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+__device__ __forceinline__ void tma_load4(uint32_t dst, const CUtensorMap* map, int x, int slot, int head, int block,
+                                          uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(slot), "r"(head), "r"(block), "r"(smem_addr(bar))
+        : "memory");
+}
+
+__device__ __forceinline__ void raw_copy(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"(smem_addr(bar))
+                 : "memory");
+}
+
+// Two floats in one register pair.
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t x) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// The largest of three; NaN where one of them is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 2^x on the FMA units for x <= 127: x = n + f by adding and taking away 1.5 * 2^23 (n then
+// stands in the low bits), 2^f as a polynomial with p(0) = 1, and n added to its exponent.
+// What is below -127 becomes exactly 0: p(0) 2^-127 has an empty exponent and fraction.
+__device__ __forceinline__ uint64_t exp2_fma(uint64_t x) {
+    const float2 v = unpair(x);
+    x = pair2(fmaxf(v.x, -127.f), fmaxf(v.y, -127.f));
+    const uint64_t r = add2(x, pair2(12582912.f, 12582912.f));
+    const uint64_t f = fma2(add2(r, pair2(-12582912.f, -12582912.f)), pair2(-1.f, -1.f), x);
+    uint64_t y = fma2(f, pair2(0.009582853f, 0.009582853f), pair2(0.055906426f, 0.055906426f));
+    y = fma2(y, f, pair2(0.240240991f, 0.240240991f));
+    y = fma2(y, f, pair2(0.693124175f, 0.693124175f));
+    y = fma2(y, f, pair2(1.f, 1.f));
+    const float2 n = unpair(r), m = unpair(y);
+    return pair2(__uint_as_float(__float_as_uint(n.x) * 0x800000u + __float_as_uint(m.x)),
+                 __uint_as_float(__float_as_uint(n.y) * 0x800000u + __float_as_uint(m.y)));
+}
+
 template <int R>
 __device__ __forceinline__ void take_registers() {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R));
@@ -158,12 +240,14 @@ __device__ __forceinline__ void give_registers() {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R));
 }
 
-template <int D>
+template <int D, bool Q4>
 struct TileBars {
-    uint64_t full[TileConfig<D>::kStages], empty[TileConfig<D>::kStages];
+    uint64_t full[TileConfig<D, Q4>::kStages], empty[TileConfig<D, Q4>::kStages];
+    uint64_t raw_full[4], raw_empty[4];
     uint64_t q_full, q_empty;
     uint64_t s_full[2], p_full[2], o_full[2];
     uint64_t drain;
+    uint32_t raw_bad[4];       // 16-key groups of a raw tile that were not copied
     uint32_t tmem;
     uint32_t abort;
 };
@@ -204,23 +288,104 @@ __device__ __forceinline__ AttnItem tile_item(const AttnParams& p, int x) {
     return it;
 }
 
+// Whether a tile of a 16-bit cache is gathered row by row: always without TMA, else the value
+// tile (odd op) that reaches behind the context.
+__device__ __forceinline__ bool gathered(int box_rows, int op, int first, int last) {
+    return box_rows == 0 || ((op & 1) && first + kTileKeys - 1 > last);
+}
+
+// The copies of one CTA, by one warp: TMA boxes of a 16-bit cache into the operand
+// ring, raw pages of a 4-bit cache into the ring of raw tiles. A lane looks up one box or run
+// of 16 keys and copies it, so that a tile's page lookups are in flight together.
+template <int D, bool Q4>
+__device__ __forceinline__ void issue_copies(const AttnParams& p, const TileMaps& maps, uint32_t base, TileBars<D, Q4>* bars,
+                                             int items) {
+    using C = TileConfig<D, Q4>;
+    Ring<Q4 ? C::kRawStages : C::kStages> ring;
+    uint32_t* abort = &bars->abort;
+    const int lane = threadIdx.x & 31;
+    const int run = Q4 ? 16 : maps.box_rows;            // keys of a copy
+    const int at = lane * run;                          // this lane's first key in a tile
+    for (int x = blockIdx.x; x < items; x += gridDim.x) {
+        const AttnItem it = tile_item(p, x);
+        const KeyTiles kt = key_tiles<kTileKeys>(p, it);
+        const int n = kt.end - kt.begin;
+        const int last = it.pos0 + it.tokens - 1;
+        const int32_t* table = p.table + it.seq * p.table_stride;
+        for (int op = 0; op < 2 * n; ++op, ring.next()) {
+            const int j = kt.first_key<kTileKeys>(kt.begin + (op >> 1)) + at;
+            if constexpr (!Q4) {
+                if (!warp_wait(&bars->empty[ring.at], ring.phase ^ 1, abort, p.status)) return;
+                if (run == 0 || gathered(run, op, j - at, last)) {
+                    if (lane == 0) mbar_arrive(&bars->full[ring.at]);
+                    continue;
+                }
+            }
+            // Keys that some row sees, in a page that exists.
+            int id = -1, slot = 0;
+            if (at < kTileKeys && j <= last && (it.pos0 - (j + run - 1) < p.window || j < p.sinks)) {
+                const int blk = block_of(p, j);
+                slot = j - blk * p.block_size;
+                id = blk < p.table_width ? table[blk] : -1;
+                if (id < 0 || id >= p.num_blocks) {
+                    atomicOr(p.status, KVX_DEV_BAD_SRC_ID);
+                    id = -1;
+                }
+            }
+            if constexpr (!Q4) {
+                uint64_t* bar = &bars->full[ring.at];
+                if (lane == 0) mbar_arrive_expect_tx(bar, C::kTileBytes);
+                __syncwarp();
+                const uint32_t tile = base + C::kRing + ring.at * C::kTileBytes;
+                // What is not to be read comes from outside the cache: zeros.
+                if (at < kTileKeys)
+#pragma unroll
+                    for (int c = 0; c < C::kSlabs; ++c)
+                        tma_load4(tile + c * C::kSlabBytes + at * 128, op & 1 ? &maps.v : &maps.k, 64 * c, slot, it.head,
+                                  id < 0 ? static_cast<int>(p.num_blocks) : id, bar);
+            } else {
+                if (!warp_wait(&bars->raw_empty[ring.at], ring.phase ^ 1, abort, p.status)) return;
+                uint64_t* bar = &bars->raw_full[ring.at];
+                const uint32_t take = __ballot_sync(~0u, id >= 0);
+                if (lane == 0) {
+                    *reinterpret_cast<volatile uint32_t*>(&bars->raw_bad[ring.at]) = ~take;
+                    mbar_arrive_expect_tx(bar, __popc(take) * 16 * (D / 2 + D / 16));
+                }
+                __syncwarp();
+                const uint32_t raw = base + C::kRaw + ring.at * C::kRawBytes;
+                if (id >= 0) {
+                    const char* src = (op & 1 ? p.v : p.k) + it.head * p.head_stride + id * p.block_stride;
+                    raw_copy(raw + at * (D / 2), src + slot * (D / 2), 16 * (D / 2), bar);
+                    raw_copy(raw + C::kRawCodes + at * (D / 16), src + p.block_size * (D / 2) + slot * (D / 16),
+                             16 * (D / 16), bar);
+                }
+            }
+        }
+    }
+}
+
 template <typename T, int D, bool Q4>
-__global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid_constant__ AttnParams p) {
-    using C = TileConfig<D>;
+__global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid_constant__ AttnParams p,
+                                                                  const __grid_constant__ TileMaps maps) {
+    using C = TileConfig<D, Q4>;
     using M = typename std::conditional<Q4, __half, T>::type;       // type of the products' operands
     extern __shared__ char raw[];
     const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
     char* smem = raw + (base - smem_addr(raw));
     float* factors = reinterpret_cast<float*>(smem + C::kFactors);  // what each query row was divided by
-    auto* bars = reinterpret_cast<TileBars<D>*>(smem + C::kBars);
+    auto* bars = reinterpret_cast<TileBars<D, Q4>*>(smem + C::kBars);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     griddep_launch_dependents();
     if (warp == 12) {
         tmem_alloc(&bars->tmem, 512);
         if (lane == 0) {
             for (int i = 0; i < C::kStages; ++i) {
-                mbar_init(&bars->full[i], 128);
+                mbar_init(&bars->full[i], Q4 ? 128 : 5);    // 16-bit: warps 8-11 and 13
                 mbar_init(&bars->empty[i], 1);
+            }
+            for (int i = 0; i < 4; ++i) {
+                mbar_init(&bars->raw_full[i], 1);
+                mbar_init(&bars->raw_empty[i], 128);
             }
             mbar_init(&bars->q_full, 128);
             mbar_init(&bars->q_empty, 1);
@@ -243,7 +408,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
     const int items = p.tile_slots * p.kv_heads * p.splits;
 
     if (warp >= 12) {
-        give_registers<40>();
+        give_registers<48>();
         if (warp == 12 && lane == 0) {
             // ---- products ----
             constexpr uint32_t qk = instruction(std::is_same<M, __nv_bfloat16>::value, false, kTileKeys);
@@ -312,11 +477,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
             bar_wait(&bars->drain, 0, &never, p.status);
         }
         __syncwarp();
+        if (warp == 13) issue_copies<D, Q4>(p, maps, base, bars, items);
     } else if (warp >= 8) {
-        give_registers<88>();
-        // ---- loads ----
+        give_registers<48>();
+        // ---- queries, edge tiles, widening ----
         const int w = warp - 8;
         Ring<C::kStages> ring;
+        Ring<Q4 ? C::kRawStages : 1> raw;
         uint32_t q_phase = 1;                                       // the first query tile is free
         constexpr int kChunks = D / 8;                              // 16-byte chunks of a row of 16-bit elements
         constexpr int kRowsPerStep = 32 / kChunks;
@@ -324,151 +491,32 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
         auto chunk_at = [](uint32_t tile, int r, int c) {
             return tile + (c >> 3) * C::kSlabBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4);
         };
-        if constexpr (!Q4) {
-            uint64_t* pending[kLag] = {};
-            int waiting = 0;                                        // loads issued and not yet announced
-            bool ok = true;
-            auto announce_oldest = [&]() {
-                fence_async_shared();
-                mbar_arrive(pending[0]);
-#pragma unroll
-                for (int i = 0; i + 1 < kLag; ++i) pending[i] = pending[i + 1];
-                --waiting;
-            };
-            auto issued = [&](uint64_t* bar) {
-                asm volatile("cp.async.commit_group;" ::: "memory");
-                if (waiting == kLag) {
-                    asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
-                    announce_oldest();
-                }
-#pragma unroll
-                for (int i = 0; i < kLag; ++i)
-                    if (i == waiting) pending[i] = bar;
-                ++waiting;
-            };
-            for (int x = blockIdx.x; x < items && ok; x += gridDim.x) {
-                const AttnItem it = tile_item(p, x);
-                const KeyTiles kt = key_tiles<kTileKeys>(p, it);
-                const int n = kt.end - kt.begin;
-                if (n <= 0) continue;
-                const int last = it.pos0 + it.tokens - 1;
-                const int32_t* table = p.table + it.seq * p.table_stride;
-                const int64_t head_off = it.head * p.head_stride;
-                const int q_after = n > 1 ? 3 : 2;                  // the queries follow this many key and value tiles
-                for (int op = 0; op <= 2 * n; ++op) {
-                    if (op == q_after) {
-                        if (!(ok = warp_wait(&bars->q_empty, q_phase, abort, p.status))) break;
-                        q_phase ^= 1;
-                        int64_t off[2];
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int r = 64 * w + 32 * h + lane, token = r / p.group;
-                            off[h] = token < it.tokens ? (it.q0 + token) * p.q_token_stride +
-                                                             (it.head * p.group + r - token * p.group) * p.q_head_stride
-                                                       : -1;
-                        }
+        bool ok = true;
+        for (int x = blockIdx.x; x < items && ok; x += gridDim.x) {
+            const AttnItem it = tile_item(p, x);
+            const KeyTiles kt = key_tiles<kTileKeys>(p, it);
+            const int n = kt.end - kt.begin;
+            if (n <= 0) continue;
+            const int last = it.pos0 + it.tokens - 1;
+            const int q_after = n > 1 ? 3 : 2;                      // the queries follow this many key and value tiles
+            for (int op = 0; op <= 2 * n; ++op) {
+                if (op == q_after) {
+                    if (!(ok = warp_wait(&bars->q_empty, q_phase, abort, p.status))) break;
+                    q_phase ^= 1;
 #pragma unroll 4
-                        for (int s = 0; s < 64; s += kRowsPerStep) {
-                            const int r = s + lane / kChunks, c = lane % kChunks;
-                            const int64_t a = __shfl_sync(~0u, s < 32 ? off[0] : off[1], r & 31);
-                            const int row = 64 * w + r;
-                            cp16(chunk_at(base + (row >> 7) * C::kTileBytes, row & 127, c), p.q + (a < 0 ? 0 : a) + 16 * c,
-                                 a >= 0);
-                        }
-                        issued(&bars->q_full);
-                    }
-                    if (op == 2 * n) break;
-                    if (!(ok = warp_wait(&bars->empty[ring.at], ring.phase ^ 1, abort, p.status))) break;
-                    const int first = kt.first_key<kTileKeys>(kt.begin + (op >> 1));
-                    const char* plane = (op & 1 ? p.v : p.k);
-                    const uint32_t tile = base + C::kRing + ring.at * C::kTileBytes;
-                    int64_t off = -1;
-                    const int j = first + 32 * w + lane;
-                    if (j <= last && (it.pos0 - j < p.window || j < p.sinks)) {
-                        const int blk = block_of(p, j);
-                        off = page_offset(p, table, blk);
-                        if (off >= 0) off += (j - blk * p.block_size) * p.slot_stride + head_off;
-                    }
-#pragma unroll 4
-                    for (int s = 0; s < 32; s += kRowsPerStep) {
-                        const int r = s + lane / kChunks, c = lane % kChunks;
-                        const int64_t a = __shfl_sync(~0u, off, r);
-                        cp16(chunk_at(tile, 32 * w + r, c), plane + (a < 0 ? 0 : a) + 16 * c, a >= 0);
-                    }
-                    issued(&bars->full[ring.at]);
-                    ring.next();
-                }
-            }
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-            if (ok)
-                while (waiting > 0) announce_oldest();
-        } else {
-            bool ok = true;
-            for (int x = blockIdx.x; x < items && ok; x += gridDim.x) {
-                const AttnItem it = tile_item(p, x);
-                const KeyTiles kt = key_tiles<kTileKeys>(p, it);
-                const int n = kt.end - kt.begin;
-                if (n <= 0) continue;
-                const int last = it.pos0 + it.tokens - 1;
-                const int32_t* table = p.table + it.seq * p.table_stride;
-                const int64_t head_off = it.head * p.head_stride;
-                const int scales_at = p.block_size * (D / 2);
-                const int q_after = n > 1 ? 3 : 2;
-                const int t = lane & 3;                             // quarter of a row: D/4 elements
-                constexpr int kWords = D / 32;                      // of codes a lane holds per key
-                // A lane's codes and scales of four keys (8 apart) of a tile.
-                uint32_t codes[4][kWords], scale[4];
-                auto fetch = [&](int op) {
-                    const int first = kt.first_key<kTileKeys>(kt.begin + (op >> 1)) + 32 * w;
-                    const char* plane = (op & 1 ? p.v : p.k);
-                    int64_t page = -1;
-                    int off = 0;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        // block_size is a multiple of 16: 16 keys from a multiple of 16 share a page.
-                        const int first16 = first + (i >> 1) * 16;
-                        if ((i & 1) == 0) {
-                            page = -1;
-                            if (first16 <= last && (it.pos0 - (first16 + 15) < p.window || first16 < p.sinks)) {
-                                const int blk = block_of(p, first16);
-                                page = page_offset(p, table, blk);
-                                off = first16 - blk * p.block_size;
-                            }
-                        }
-                        const int key = (i & 1) * 8 + (lane >> 2), j = first16 + key;
-                        scale[i] = 0;
-#pragma unroll
-                        for (int k = 0; k < kWords; ++k) codes[i][k] = 0;
-                        if (page >= 0 && j <= last && (it.pos0 - j < p.window || j < p.sinks)) {
-                            const char* b = plane + page + head_off;
-                            const char* c = b + (off + key) * (D / 2) + t * (D / 8);
-                            const char* s = b + scales_at + (off + key) * (D / 16);
-                            if constexpr (D == 128) {
-                                const uint4 v = __ldg(reinterpret_cast<const uint4*>(c));
-                                codes[i][0] = v.x, codes[i][1] = v.y, codes[i][2] = v.z, codes[i][3] = v.w;
-                                scale[i] = __ldg(reinterpret_cast<const uint16_t*>(s) + t);
-                            } else {
-                                const uint2 v = __ldg(reinterpret_cast<const uint2*>(c));
-                                codes[i][0] = v.x, codes[i][1] = v.y;
-                                scale[i] = __ldg(reinterpret_cast<const uint8_t*>(s) + t);
-                            }
-                        }
-                    }
-                };
-                fetch(0);
-                for (int op = 0; op <= 2 * n; ++op) {
-                    if (op == q_after) {
-                        if (!(ok = warp_wait(&bars->q_empty, q_phase, abort, p.status))) break;
-                        q_phase ^= 1;
-#pragma unroll 2
-                        for (int s = 0; s < 64; s += kRowsPerStep) {
-                            const int row = 64 * w + s + lane / kChunks, c = lane % kChunks;
-                            const int token = row / p.group;
-                            uint4 v = make_uint4(0, 0, 0, 0);
-                            if (token < it.tokens)
-                                v = *reinterpret_cast<const uint4*>(
-                                    p.q + (it.q0 + token) * p.q_token_stride +
-                                    (it.head * p.group + row - token * p.group) * p.q_head_stride + 16 * c);
+                    for (int s = 0; s < 64; s += kRowsPerStep) {
+                        const int row = 64 * w + s + lane / kChunks, c = lane % kChunks;
+                        const int token = row / p.group;
+                        const bool take = token < it.tokens;
+                        const char* src = p.q + 16 * c +
+                                          (take ? (it.q0 + token) * p.q_token_stride +
+                                                      (it.head * p.group + row - token * p.group) * p.q_head_stride
+                                                : 0);
+                        const uint32_t dst = chunk_at(base + (row >> 7) * C::kTileBytes, row & 127, c);
+                        if constexpr (!Q4) {
+                            cp16(dst, src, take);
+                        } else {
+                            uint4 v = take ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
                             float factor = 1.f;
                             if constexpr (!std::is_same<T, __half>::value) {
                                 const float2 a = Pair<T>::unpack(v.x), b = Pair<T>::unpack(v.y), d = Pair<T>::unpack(v.z),
@@ -484,45 +532,95 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                                 v.z = Pair<__half>::pack(d.x * inv, d.y * inv);
                                 v.w = Pair<__half>::pack(e.x * inv, e.y * inv);
                             }
-                            st_shared16(chunk_at(base + (row >> 7) * C::kTileBytes, row & 127, c), v.x, v.y, v.z, v.w);
+                            st_shared16(dst, v.x, v.y, v.z, v.w);
                             if (c == 0) factors[row] = factor;
                         }
-                        fence_async_shared();
-                        mbar_arrive(&bars->q_full);
                     }
-                    if (op == 2 * n) break;
-                    uint32_t now[4][kWords], now_scale[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        now_scale[i] = scale[i];
-#pragma unroll
-                        for (int k = 0; k < kWords; ++k) now[i][k] = codes[i][k];
-                    }
-                    if (op + 1 < 2 * n) fetch(op + 1);
+                    if constexpr (!Q4) asm volatile("cp.async.wait_all;" ::: "memory");
+                    fence_async_shared();
+                    mbar_arrive(&bars->q_full);
+                }
+                if (op == 2 * n) break;
+                const int first = kt.first_key<kTileKeys>(kt.begin + (op >> 1));
+                const uint32_t tile = base + C::kRing + ring.at * C::kTileBytes;
+                if constexpr (!Q4) {
+                    // Warp 13 and these four go through every stage together, whichever of them fills it: a
+                    // barrier's phases are told apart by parity alone, so none may fall two behind.
                     if (!(ok = warp_wait(&bars->empty[ring.at], ring.phase ^ 1, abort, p.status))) break;
-                    const uint32_t tile = base + C::kRing + ring.at * C::kTileBytes;
+                    if (gathered(maps.box_rows, op, first, last)) {
+                        int64_t off = -1;
+                        const int j = first + 32 * w + lane;
+                        if (j <= last && (it.pos0 - j < p.window || j < p.sinks)) {
+                            const int blk = block_of(p, j);
+                            off = page_offset(p, p.table + it.seq * p.table_stride, blk);
+                            if (off >= 0) off += (j - blk * p.block_size) * p.slot_stride + it.head * p.head_stride;
+                        }
+                        const char* plane = op & 1 ? p.v : p.k;
+#pragma unroll 4
+                        for (int s = 0; s < 32; s += kRowsPerStep) {
+                            const int r = s + lane / kChunks, c = lane % kChunks;
+                            const int64_t a = __shfl_sync(~0u, off, r);
+                            cp16(chunk_at(tile, 32 * w + r, c), plane + (a < 0 ? 0 : a) + 16 * c, a >= 0);
+                        }
+                        asm volatile("cp.async.wait_all;" ::: "memory");
+                        fence_async_shared();
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars->full[ring.at]);
+                } else {
+                    if (!(ok = warp_wait(&bars->raw_full[raw.at], raw.phase, abort, p.status))) break;
+                    if (!(ok = warp_wait(&bars->empty[ring.at], ring.phase ^ 1, abort, p.status))) break;
+                    const uint32_t from = base + C::kRaw + raw.at * C::kRawBytes;
+                    const uint32_t bad = *reinterpret_cast<volatile uint32_t*>(&bars->raw_bad[raw.at]);
+                    const int t = lane & 3;                         // quarter of a row: D/4 elements
+                    constexpr int kWords = D / 32;                  // of codes a lane holds per key
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int row = 32 * w + 8 * i + (lane >> 2);
-                        const uint32_t lo = now_scale[i] & 0xff, hi = D == 128 ? now_scale[i] >> 8 : lo;
-                        const uint32_t s2[2] = {scales_to_half(lo | (lo << 8)), scales_to_half(hi | (hi << 8))};
+                        const int row = 32 * w + 8 * i + (lane >> 2), j = first + row;
+                        uint32_t codes[kWords], scale;
+                        // The right half of the row's words comes first in lanes 2 and 3 of a row: the 16-byte
+                        // stores of eight lanes then fall on eight different bank groups.
+                        const int flip = D == 128 ? (t >> 1) * 2 : 0;
+                        const uint32_t at = from + row * (D / 2) + t * (D / 8);
+                        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(codes[0]), "=r"(codes[1]) : "r"(at + flip * 4));
+                        if constexpr (D == 128) {
+                            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
+                                         : "=r"(codes[2]), "=r"(codes[3])
+                                         : "r"(at + (flip ^ 2) * 4));
+                            uint16_t u;
+                            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(from + C::kRawCodes + row * 8 + t * 2));
+                            scale = u;
+                        } else {
+                            uint16_t u;
+                            asm volatile("ld.shared.u8 %0, [%1];" : "=h"(u) : "r"(from + C::kRawCodes + row * 4 + t));
+                            scale = u;
+                        }
+                        // Keys that no row sees and bad pages read as zeros, whatever the raw tile holds.
+                        const bool take = !((bad >> (row >> 4)) & 1) && j <= last && (it.pos0 - j < p.window || j < p.sinks);
+                        if (!take) scale = 0;
+                        const uint32_t lo = scale & 0xff, hi = D == 128 ? scale >> 8 : lo;
+                        const uint32_t s_lo = scales_to_half(lo | (lo << 8)), s_hi = scales_to_half(hi | (hi << 8));
 #pragma unroll
                         for (int k = 0; k < kWords; ++k) {
                             uint32_t h[4];
-                            codes_to_half(now[i][k], h);
-                            const uint32_t s = s2[D == 128 ? k / 2 : 0];
-                            st_shared16(chunk_at(tile, row, t * kWords + k), mul_half2(h[0], s), mul_half2(h[1], s),
+                            codes_to_half(codes[k], h);
+                            const int word = k ^ flip;              // words 0, 1: first 16 elements, 2, 3: the others
+                            const uint32_t s = D == 128 && (word & 2) ? s_hi : s_lo;
+                            st_shared16(chunk_at(tile, row, t * kWords + word), mul_half2(h[0], s), mul_half2(h[1], s),
                                         mul_half2(h[2], s), mul_half2(h[3], s));
                         }
                     }
+                    mbar_arrive(&bars->raw_empty[raw.at]);
+                    raw.next();
                     fence_async_shared();
                     mbar_arrive(&bars->full[ring.at]);
-                    ring.next();
                 }
+                ring.next();
             }
         }
+        if constexpr (!Q4) asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
-        take_registers<192>();
+        take_registers<208>();
         // ---- softmax ----
         const int i = warp >> 2;                                    // row tile
         const int row = (threadIdx.x & 127) + i * kHalfRows;        // row of the item
@@ -571,15 +669,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                     for (int c = 0; c < kTileKeys; ++c)
                         if (c > hi || (c < lo && c >= head_cols)) sr[c] = __float_as_uint(-INFINITY);
                 }
-                float next = top;
+                // Four chains of three-way maxima. A NaN among the scores makes the row's result NaN.
+                float best[4] = {top, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 0; c < kTileKeys; ++c) next = fmaxf(next, __uint_as_float(sr[c]));
+                for (int c = 0; c < kTileKeys; c += 8)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        best[k] = max3(best[k], __uint_as_float(sr[c + 2 * k]), __uint_as_float(sr[c + 2 * k + 1]));
+                const float next = max3(max3(best[0], best[1], best[2]), best[3], best[3]);
                 // Keep the old maximum while weights stay below 2^8.
-                const bool grow = j == 0 || (next - top) * scale > 8.f || top == -INFINITY;
+                const bool grow = j == 0 || !((next - top) * scale <= 8.f);
                 const float old = top;
                 if (grow) top = next;
-                const float ref = top == -INFINITY ? 0.f : top * scale;
-                if (j > 0 && __any_sync(~0u, grow && next > old)) {
+                // An infinite score gives NaN, as inf - inf does in the formula.
+                const float ref = top == -INFINITY ? 0.f : top == INFINITY ? NAN : top * scale;
+                if (j > 0 && __any_sync(~0u, grow && next != old)) {
                     const float shrink = old == -INFINITY ? 0.f : exp2_approx(old * scale - ref);
                     sum *= shrink;
 #pragma unroll
@@ -592,21 +696,30 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                         tmem_store32(o_at + c, o);
                     }
                 }
-                float part[4] = {0.f, 0.f, 0.f, 0.f};
+                uint64_t part[2] = {0, 0};
+                const uint64_t scale2 = pair2(scale, scale), ref2 = pair2(-ref, -ref);
 #pragma unroll
                 for (int c = 0; c < kTileKeys; c += 32) {
                     uint32_t w[16];
 #pragma unroll
-                    for (int k = 0; k < 32; k += 2) {
-                        const float a = exp2_approx(fmaf(__uint_as_float(sr[c + k]), scale, -ref));
-                        const float b = exp2_approx(fmaf(__uint_as_float(sr[c + k + 1]), scale, -ref));
-                        part[k & 2] += a;
-                        part[(k & 2) + 1] += b;
-                        w[k / 2] = Pair<M>::pack(a, b);
+                    for (int k = 0; k < 16; ++k) {
+                        const uint64_t e = fma2(pair2(__uint_as_float(sr[c + 2 * k]), __uint_as_float(sr[c + 2 * k + 1])),
+                                                scale2, ref2);
+                        uint64_t y;
+                        if ((k & 7) < kFmaPairs) {
+                            y = exp2_fma(e);
+                        } else {
+                            const float2 v = unpair(e);
+                            y = pair2(exp2_approx(v.x), exp2_approx(v.y));
+                        }
+                        part[k & 1] = add2(part[k & 1], y);
+                        const float2 v = unpair(y);
+                        w[k] = Pair<M>::pack(v.x, v.y);
                     }
                     tmem_store16(s_at + c / 2, w);
                 }
-                sum += (part[0] + part[1]) + (part[2] + part[3]);
+                const float2 total = unpair(add2(part[0], part[1]));
+                sum += total.x + total.y;
                 tc_wait_st();
                 tc_fence_before();
                 mbar_arrive(&bars->p_full[i]);
@@ -664,13 +777,58 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    // After a wait that ran out, copies may still be on their way into this CTA's shared memory: 1 ms is
+    // a thousand times what one takes.
+    if (*reinterpret_cast<volatile uint32_t*>(abort))
+        for (int i = 0; i < 1000; ++i) __nanosleep(1000);
     if (warp == 12) tmem_free(tmem, 512);
+}
+
+// cuTensorMapEncodeTiled, from the driver that is loaded.
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static int encode_maps(const AttnParams& p, int head_dim, bool bf16, TileMaps* maps) {
+    maps->box_rows = 0;
+    int rows = p.block_size & -p.block_size;            // the largest power of two that divides a page
+    if (rows < 8) return KVX_OK;                        // the swizzle repeats every 8 rows
+    rows = rows > kTileKeys ? kTileKeys : rows;
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(p.slot_stride), static_cast<cuuint64_t>(p.head_stride),
+                                   static_cast<cuuint64_t>(p.block_stride)};
+    for (const cuuint64_t st : strides)
+        if (st == 0 || st >= (1ull << 40)) return KVX_OK;     // also negative ones
+    if (p.num_blocks > 0x7fffffff) return KVX_OK;
+    static std::atomic<EncodeTiled> encode{nullptr};
+    EncodeTiled fn = encode.load(std::memory_order_acquire);
+    if (fn == nullptr) {
+        void* sym = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        KVX_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &sym, 12000, cudaEnableDefault, &found),
+                 "find cuTensorMapEncodeTiled");
+        if (sym == nullptr) return fail(KVX_ECUDA, "cuTensorMapEncodeTiled not available from the driver");
+        fn = reinterpret_cast<EncodeTiled>(sym);
+        encode.store(fn, std::memory_order_release);
+    }
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(p.block_size),
+                                static_cast<cuuint64_t>(p.kv_heads), static_cast<cuuint64_t>(p.num_blocks)};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(rows), 1, 1}, steps[4] = {1, 1, 1, 1};
+    for (int i = 0; i < 2; ++i) {
+        const CUresult r = fn(i ? &maps->v : &maps->k,
+                              bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                              const_cast<char*>(i ? p.v : p.k), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (r != CUDA_SUCCESS) return KVX_OK;           // a layout that TMA does not take is gathered
+    }
+    maps->box_rows = rows;
+    return KVX_OK;
 }
 
 template <typename T, int D, bool Q4>
 static int run_tile(const AttnParams& p, int device, int sms, cudaStream_t stream) {
-    constexpr int smem = TileConfig<D>::kSmem;
-    static_assert(smem <= 227 * 1024 && sizeof(TileBars<D>) <= 256, "shared memory of the tile kernel");
+    constexpr int smem = TileConfig<D, Q4>::kSmem;
+    static_assert(smem <= 227 * 1024 && sizeof(TileBars<D, Q4>) <= 512, "shared memory of the tile kernel");
     static std::atomic<uint64_t> done{0};               // devices that have the opt-in
     const uint64_t bit = 1ull << device;
     if (!(done.load(std::memory_order_relaxed) & bit)) {
@@ -684,6 +842,11 @@ static int run_tile(const AttnParams& p, int device, int sms, cudaStream_t strea
     }
     const int64_t items = static_cast<int64_t>(p.tile_slots) * p.kv_heads * p.splits;
     if (items > INT_MAX) return fail(KVX_EUNSUPPORTED, "too many tiles of queries for one call");
+    TileMaps maps = {};
+    if (!Q4) {
+        const int rc = encode_maps(p, D, std::is_same<T, __nv_bfloat16>::value, &maps);
+        if (rc != KVX_OK) return rc;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(items < sms ? items : sms));
     cfg.blockDim = dim3(kTileThreads);
@@ -694,7 +857,7 @@ static int run_tile(const AttnParams& p, int device, int sms, cudaStream_t strea
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    KVX_CUDA(cudaLaunchKernelEx(&cfg, attn_tile_kernel<T, D, Q4>, p), "launch attention kernel");
+    KVX_CUDA(cudaLaunchKernelEx(&cfg, attn_tile_kernel<T, D, Q4>, p, maps), "launch attention kernel");
     return KVX_OK;
 }
 

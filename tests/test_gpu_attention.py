@@ -8,8 +8,9 @@ compared bit for bit. Attention is held, element by element, to
 u_out: half a step of the output type. u_w: half a step of the 16-bit type the
 weights are rounded to (bf16 2^-8, fp16 and 4-bit caches 2^-11; the error of the
 sum in the denominator is covered by counting it twice). u_s: fp32 arithmetic:
-scores have D products and sums of magnitude up to `reach`, exponentials 2^-22
-and their argument's rounding, sums n terms: 2^-24 (2 (D + 8) reach + n + 16), in
+scores have D products and sums of magnitude up to `reach`, exponentials 2.8e-6 <
+48 * 2^-24 (a degree-4 polynomial; the special-function unit's 2^-22 is less) and
+their argument's rounding, sums n terms: 2^-24 (2 (D + 8) reach + n + 64), in
 numerator and denominator alike. The last term is what fp16 weights below its
 smallest normal number lose (2^-25 of the largest weight each).
 """
@@ -31,7 +32,7 @@ HALF_STEP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 
 def bound(want: ref.Attended, dtype, q4: bool, dim: int) -> torch.Tensor:
     u_w = 2 * (2.0 ** -11 if q4 else HALF_STEP[dtype])
-    u_s = 2 * 2.0 ** -24 * (2 * (dim + 8) * want.reach + want.keys + 16)
+    u_s = 2 * 2.0 ** -24 * (2 * (dim + 8) * want.reach + want.keys + 64)
     return HALF_STEP[dtype] * want.out.abs() + (u_w + u_s) * want.mass + want.keys * 2.0 ** -25 * want.top
 
 
