@@ -376,7 +376,7 @@ int kvx_load_kvcache_q4(int32_t device, int32_t dtype, void* key_dev, void* valu
  * All device reads of lengths, tables and data follow earlier work on `stream`;
  * nothing is read on the host, so the call can be captured and replayed with
  * other lengths. `workspace_dev` holds partial results where the keys are split
- * (kvx_attention_workspace bytes, 16-byte aligned; may be NULL when that is 0);
+ * (kvx_attention_workspace bytes, 32-byte aligned; may be NULL when that is 0);
  * calls that overlap need workspaces of their own. */
 typedef struct kvx_attention {
     uint64_t query, out;             /* [num_tokens, num_heads, head_dim], 16-bit */

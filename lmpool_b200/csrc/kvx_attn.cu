@@ -132,6 +132,7 @@ int kvx_paged_attention(int32_t device, const kvx_attention* args, void* workspa
     if (a.cache_bits == 16)
         bits |= static_cast<uint64_t>(a.cache_slot_stride) | static_cast<uint64_t>(a.cache_head_stride);
     if (bits & 15) return fail(KVX_EINVAL, "addresses and strides must be multiples of 16 bytes");
+    if (reinterpret_cast<uint64_t>(workspace_dev) & 31) return fail(KVX_EINVAL, "workspace_dev must be 32-byte aligned");
     int sms = 0;
     rc = sm_count(device, &sms);
     if (rc != KVX_OK) return rc;
@@ -174,6 +175,7 @@ int kvx_paged_attention(int32_t device, const kvx_attention* args, void* workspa
     p.splits = pl.splits;
     p.tile_tokens = pl.tile_tokens;
     p.tile_slots = pl.tile_slots;
+    p.out_wide = ((a.out | static_cast<uint64_t>(a.out_token_stride) | static_cast<uint64_t>(a.out_head_stride)) & 31) == 0;
     if (pl.splits > 1) {
         p.ws_o = static_cast<float*>(workspace_dev);
         p.ws_ml = p.ws_o + static_cast<int64_t>(a.num_tokens) * a.num_heads * pl.splits * a.head_dim;

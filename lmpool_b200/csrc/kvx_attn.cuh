@@ -43,6 +43,7 @@ struct AttnParams {
     int32_t splits;
     int32_t tile_tokens;                      // tokens of an item
     int32_t tile_slots;                       // item slots per (kv head, split)
+    int32_t out_wide;                         // output rows start at multiples of 32 bytes
 };
 
 struct AttnItem {

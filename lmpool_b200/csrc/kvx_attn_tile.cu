@@ -8,7 +8,8 @@
 //   0-3, 4-7  softmax of row tile 0 and 1: a thread owns a row;
 //   8-11      queries into shared memory; edge tiles of a 16-bit cache; widening of a 4-bit one;
 //   12        one thread issues the products;
-//   13        issues the bulk copies (14, 15 idle).
+//   13        issues the bulk copies;
+//   14        looks up items ahead (lengths, offsets, ranges of keys; 15 idle).
 // Tensor memory (512 columns): S0, S1 (128 fp32 columns each), O0, O1 (D each).
 // The weights P overwrite the first half of their S as 16-bit pairs and are the A
 // operand of O += P V straight from tensor memory. Per row tile i and key tile j the
@@ -69,7 +70,7 @@ struct TileConfig {
     static constexpr int kRaw = kRing + kStages * kTileBytes;
     static constexpr int kFactors = kRaw + kRawStages * kRawBytes;
     static constexpr int kBars = kFactors + 2 * kHalfRows * 4;
-    static constexpr int kSmem = 1024 + kBars + 512;
+    static constexpr int kSmem = 1024 + kBars + 768;
 };
 
 // TMA views of a 16-bit cache: [D, block_size, kv_heads, num_blocks] from the innermost.
@@ -102,6 +103,12 @@ __device__ __forceinline__ void tc_wait_ld(uint32_t* r) {
 }
 __device__ __forceinline__ void after_wait_ld(uint32_t* r) { asm volatile("" : KVX_REGS32(r)::"memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// One lane of the (converged) warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
 // Arrives at `bar` when every product issued so far by this thread is done.
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
@@ -133,15 +140,17 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t* r) {
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr));
 }
-__device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t* r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
+__device__ __forceinline__ void tmem_load8(uint32_t addr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(addr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])::"memory");
+}
+__device__ __forceinline__ void tmem_store8(uint32_t addr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t* r) {
     asm volatile(
@@ -169,6 +178,16 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool take) {
 }
 __device__ __forceinline__ void st_shared16(uint32_t dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared16(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
 }
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -214,6 +233,17 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
+// 32 bytes of one row: a whole memory sector where the address allows it.
+__device__ __forceinline__ void store32(void* p, const uint32_t* r, bool wide) {
+    if (wide) {
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                     "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                     : "memory");
+    } else {
+        reinterpret_cast<uint4*>(p)[0] = make_uint4(r[0], r[1], r[2], r[3]);
+        reinterpret_cast<uint4*>(p)[1] = make_uint4(r[4], r[5], r[6], r[7]);
+    }
+}
 // 2^x on the FMA units for x <= 127: x = n + f by adding and taking away 1.5 * 2^23 (n then
 // stands in the low bits), 2^f as a polynomial with p(0) = 1, and n added to its exponent.
 // What is below -127 becomes exactly 0: p(0) 2^-127 has an empty exponent and fraction.
@@ -240,6 +270,14 @@ __device__ __forceinline__ void give_registers() {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R));
 }
 
+// An item with its keys, as warp 14 hands it to the others.
+struct TileWork {
+    AttnItem it;
+    KeyTiles kt;
+};
+constexpr int kWork = 4;       // items looked up ahead
+constexpr int kRoles = 14;     // warps that take each item: 0-13
+
 template <int D, bool Q4>
 struct TileBars {
     uint64_t full[TileConfig<D, Q4>::kStages], empty[TileConfig<D, Q4>::kStages];
@@ -247,6 +285,8 @@ struct TileBars {
     uint64_t q_full, q_empty;
     uint64_t s_full[2], p_full[2], o_full[2];
     uint64_t drain;
+    uint64_t work_full[kWork], work_empty[kWork];
+    TileWork work[kWork];
     uint32_t raw_bad[4];       // 16-key groups of a raw tile that were not copied
     uint32_t tmem;
     uint32_t abort;
@@ -288,6 +328,20 @@ __device__ __forceinline__ AttnItem tile_item(const AttnParams& p, int x) {
     return it;
 }
 
+// Writes a row again from its visible keys alone (see visible_keys_only).
+template <typename T, int D, bool Q4>
+__device__ __noinline__ void visible_row(const AttnParams& p, const AttnItem& it, const KeyTiles& kt, int tile_keys, int row,
+                                         float m2, float inv, char* dst, int64_t at) {
+    for (int c = 0; c < D; c += 32) {
+        float v[32];
+        visible_keys_only<T, D, Q4, 32>(p, it, kt, tile_keys, row, m2, c, v);
+        for (int k = 0; k < 32; ++k) {
+            if (p.splits > 1) p.ws_o[at * D + c + k] = v[k];
+            else reinterpret_cast<T*>(dst)[c + k] = static_cast<T>(v[k] * inv);
+        }
+    }
+}
+
 // Whether a tile of a 16-bit cache is gathered row by row: always without TMA, else the value
 // tile (odd op) that reaches behind the context.
 __device__ __forceinline__ bool gathered(int box_rows, int op, int first, int last) {
@@ -306,9 +360,11 @@ __device__ __forceinline__ void issue_copies(const AttnParams& p, const TileMaps
     const int lane = threadIdx.x & 31;
     const int run = Q4 ? 16 : maps.box_rows;            // keys of a copy
     const int at = lane * run;                          // this lane's first key in a tile
+    Ring<kWork> work;
     for (int x = blockIdx.x; x < items; x += gridDim.x) {
-        const AttnItem it = tile_item(p, x);
-        const KeyTiles kt = key_tiles<kTileKeys>(p, it);
+        AttnItem it;
+        KeyTiles kt;
+        if (!take_work(bars, work, p.status, it, kt)) return;
         const int n = kt.end - kt.begin;
         const int last = it.pos0 + it.tokens - 1;
         const int32_t* table = p.table + it.seq * p.table_stride;
@@ -364,6 +420,18 @@ __device__ __forceinline__ void issue_copies(const AttnParams& p, const TileMaps
     }
 }
 
+// The next item of a role (a whole warp), copied out of the ring that warp 14 fills.
+template <int D, bool Q4>
+__device__ __forceinline__ bool take_work(TileBars<D, Q4>* bars, Ring<kWork>& ring, int32_t* status, AttnItem& it, KeyTiles& kt) {
+    if (!warp_wait(&bars->work_full[ring.at], ring.phase, &bars->abort, status)) return false;
+    it = bars->work[ring.at].it;
+    kt = bars->work[ring.at].kt;
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&bars->work_empty[ring.at]);
+    ring.next();
+    return true;
+}
+
 template <typename T, int D, bool Q4>
 __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid_constant__ AttnParams p,
                                                                   const __grid_constant__ TileMaps maps) {
@@ -395,6 +463,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                 mbar_init(&bars->o_full[i], 1);
             }
             mbar_init(&bars->drain, 1);
+            for (int i = 0; i < kWork; ++i) {
+                mbar_init(&bars->work_full[i], 1);
+                mbar_init(&bars->work_empty[i], kRoles);
+            }
             bars->abort = 0;
             mbar_init_fence();
         }
@@ -407,79 +479,111 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
     uint32_t* abort = &bars->abort;
     const int items = p.tile_slots * p.kv_heads * p.splits;
 
+    // Registers: 4 x 128 a thread at launch, 2 x 208 + 56 + 40 from here on.
     if (warp >= 12) {
-        give_registers<48>();
-        if (warp == 12 && lane == 0) {
-            // ---- products ----
+        give_registers<40>();
+        if (warp == 12) {
+            // ---- products ---- (the whole warp keeps step, so that addresses stay uniform; one lane issues)
             constexpr uint32_t qk = instruction(std::is_same<M, __nv_bfloat16>::value, false, kTileKeys);
             constexpr uint32_t pv = instruction(std::is_same<M, __nv_bfloat16>::value, true, D);
+            const bool leader = elect_one();
+            const uint64_t q_desc = operand(base, 16), k_desc = operand(base + C::kRing, 16),
+                           v_desc = operand(base + C::kRing, C::kSlabBytes);
             Ring<C::kStages> ring;
             uint32_t q_phase = 0, p_phase = 0;
             auto scores = [&](int i, int stage) {
-                const uint32_t a = base + i * C::kTileBytes, b = base + C::kRing + stage * C::kTileBytes;
+                if (leader) {
+                    const uint64_t a = q_desc + i * (C::kTileBytes >> 4), b = k_desc + stage * (C::kTileBytes >> 4);
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint32_t off = (k / 4) * C::kSlabBytes + (k % 4) * 32;
-                    tc_mma_ss(tmem + i * kTileKeys, operand(a + off, 16), operand(b + off, 16), qk, k > 0);
+                    for (int k = 0; k < D / 16; ++k) {
+                        constexpr int kPerSlab = 4;
+                        const int off = ((k / kPerSlab) * C::kSlabBytes + (k % kPerSlab) * 32) >> 4;
+                        tc_mma_ss(tmem + i * kTileKeys, a + off, b + off, qk, k > 0);
+                    }
+                    tc_commit(&bars->s_full[i]);
                 }
-                tc_commit(&bars->s_full[i]);
+                __syncwarp();
             };
+            auto commit = [&](uint64_t* bar) {
+                if (leader) tc_commit(bar);
+                __syncwarp();
+            };
+            Ring<kWork> work;
             for (int x = blockIdx.x; x < items; x += gridDim.x) {
-                const AttnItem it = tile_item(p, x);
-                const KeyTiles kt = key_tiles<kTileKeys>(p, it);
+                AttnItem it;
+                KeyTiles kt;
+                if (!take_work(bars, work, p.status, it, kt)) break;
                 const int n = kt.end - kt.begin;
                 if (n <= 0) continue;
-                if (!bar_wait(&bars->q_full, q_phase, abort, p.status)) break;
+                if (!warp_wait(&bars->q_full, q_phase, abort, p.status)) break;
                 q_phase ^= 1;
-                if (!bar_wait(&bars->full[ring.at], ring.phase, abort, p.status)) break;
+                if (!warp_wait(&bars->full[ring.at], ring.phase, abort, p.status)) break;
                 tc_fence_after();
                 scores(0, ring.at);
                 scores(1, ring.at);
-                tc_commit(&bars->empty[ring.at]);
+                commit(&bars->empty[ring.at]);
+                if (n == 1) commit(&bars->q_empty);
                 ring.next();
                 bool ok = true;
                 for (int j = 0; j < n && ok; ++j) {
                     const Ring<C::kStages> v = ring;
                     ring.next();
-                    if (!(ok = bar_wait(&bars->full[v.at], v.phase, abort, p.status))) break;
-                    for (int i = 0; i < 2 && ok; ++i) {
-                        if (!(ok = bar_wait(&bars->p_full[i], p_phase, abort, p.status))) break;
-                        tc_fence_after();
-                        const uint32_t b = base + C::kRing + v.at * C::kTileBytes;
+                    if (!(ok = warp_wait(&bars->full[v.at], v.phase, abort, p.status))) break;
 #pragma unroll
-                        for (int k = 0; k < kTileKeys / 16; ++k)
-                            tc_mma_ts(tmem + 256 + i * D, tmem + i * kTileKeys + k * 8,
-                                      operand(b + k * 2048, C::kSlabBytes), pv, j > 0 || k > 0);
+                    for (int i = 0; i < 2; ++i) {
+                        if (!(ok = warp_wait(&bars->p_full[i], p_phase, abort, p.status))) break;
+                        tc_fence_after();
+                        if (leader) {
+                            const uint64_t b = v_desc + v.at * (C::kTileBytes >> 4);
+#pragma unroll
+                            for (int k = 0; k < kTileKeys / 16; ++k)
+                                tc_mma_ts(tmem + 256 + i * D, tmem + i * kTileKeys + k * 8, b + k * (2048 >> 4), pv,
+                                          j > 0 || k > 0);
+                        }
+                        __syncwarp();
                         if (j + 1 < n) {
                             if (i == 0) {
-                                if (!(ok = bar_wait(&bars->full[ring.at], ring.phase, abort, p.status))) break;
+                                if (!(ok = warp_wait(&bars->full[ring.at], ring.phase, abort, p.status))) break;
                                 tc_fence_after();
                             }
                             scores(i, ring.at);
                         } else {
-                            tc_commit(&bars->o_full[i]);
+                            commit(&bars->o_full[i]);
                         }
                     }
                     if (!ok) break;
                     p_phase ^= 1;
-                    tc_commit(&bars->empty[v.at]);
+                    commit(&bars->empty[v.at]);
                     if (j + 1 < n) {
-                        tc_commit(&bars->empty[ring.at]);
+                        commit(&bars->empty[ring.at]);
                         ring.next();
+                        if (j + 2 == n) commit(&bars->q_empty);      // no product reads these queries any more
                     }
                 }
                 if (!ok) break;
-                tc_commit(&bars->q_empty);
             }
             // Nothing of this CTA is in flight when its tensor memory is freed.
-            tc_commit(&bars->drain);
+            commit(&bars->drain);
             uint32_t never = 0;
             bar_wait(&bars->drain, 0, &never, p.status);
         }
         __syncwarp();
         if (warp == 13) issue_copies<D, Q4>(p, maps, base, bars, items);
+        if (warp == 14) {
+            Ring<kWork> ring;
+            for (int x = blockIdx.x; x < items; x += gridDim.x, ring.next()) {
+                const AttnItem it = tile_item(p, x);
+                const KeyTiles kt = key_tiles<kTileKeys>(p, it);
+                if (!warp_wait(&bars->work_empty[ring.at], ring.phase ^ 1, abort, p.status)) break;
+                if (lane == 0) {
+                    bars->work[ring.at].it = it;
+                    bars->work[ring.at].kt = kt;
+                    mbar_arrive(&bars->work_full[ring.at]);
+                }
+            }
+        }
     } else if (warp >= 8) {
-        give_registers<48>();
+        give_registers<56>();
         // ---- queries, edge tiles, widening ----
         const int w = warp - 8;
         Ring<C::kStages> ring;
@@ -491,10 +595,19 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
         auto chunk_at = [](uint32_t tile, int r, int c) {
             return tile + (c >> 3) * C::kSlabBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4);
         };
+        int my_token[2], my_head[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int row = 64 * w + 32 * h + lane;
+            my_token[h] = row / p.group;
+            my_head[h] = row - my_token[h] * p.group;
+        }
         bool ok = true;
+        Ring<kWork> work;
         for (int x = blockIdx.x; x < items && ok; x += gridDim.x) {
-            const AttnItem it = tile_item(p, x);
-            const KeyTiles kt = key_tiles<kTileKeys>(p, it);
+            AttnItem it;
+            KeyTiles kt;
+            if (!take_work(bars, work, p.status, it, kt)) break;
             const int n = kt.end - kt.begin;
             if (n <= 0) continue;
             const int last = it.pos0 + it.tokens - 1;
@@ -503,40 +616,53 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                 if (op == q_after) {
                     if (!(ok = warp_wait(&bars->q_empty, q_phase, abort, p.status))) break;
                     q_phase ^= 1;
+                    int64_t off[2];                                 // of rows 64 w + lane and 32 further
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        off[h] = my_token[h] < it.tokens ? (it.q0 + my_token[h]) * p.q_token_stride +
+                                                               (it.head * p.group + my_head[h]) * p.q_head_stride
+                                                         : -1;
 #pragma unroll 4
                     for (int s = 0; s < 64; s += kRowsPerStep) {
                         const int row = 64 * w + s + lane / kChunks, c = lane % kChunks;
-                        const int token = row / p.group;
-                        const bool take = token < it.tokens;
-                        const char* src = p.q + 16 * c +
-                                          (take ? (it.q0 + token) * p.q_token_stride +
-                                                      (it.head * p.group + row - token * p.group) * p.q_head_stride
-                                                : 0);
-                        const uint32_t dst = chunk_at(base + (row >> 7) * C::kTileBytes, row & 127, c);
-                        if constexpr (!Q4) {
-                            cp16(dst, src, take);
-                        } else {
-                            uint4 v = take ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
-                            float factor = 1.f;
-                            if constexpr (!std::is_same<T, __half>::value) {
+                        const int64_t from = __shfl_sync(~0u, s < 32 ? off[0] : off[1], row & 31);
+                        const bool take = from >= 0;
+                        const char* src = p.q + 16 * c + (take ? from : 0);
+                        cp16(chunk_at(base + (row >> 7) * C::kTileBytes, row & 127, c), src, take);
+                    }
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    if constexpr (Q4 && !std::is_same<T, __half>::value) {
+                        // To fp16 in place, a lane a row: the largest magnitude first (bf16 bits without their sign are
+                        // ordered as numbers), then the elements over its power of two.
+                        __syncwarp();
+#pragma unroll 1
+                        for (int s = 0; s < 64; s += 32) {
+                            const int row = 64 * w + s + lane;
+                            const uint32_t tile = base + (row >> 7) * C::kTileBytes;
+                            uint32_t big = 0;
+#pragma unroll 4
+                            for (int c = 0; c < kChunks; ++c) {
+                                const uint4 v = ld_shared16(chunk_at(tile, row & 127, c));
+                                big = max_u16x2(big, max_u16x2(max_u16x2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
+                                                               max_u16x2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
+                            }
+                            const uint32_t most = max(big & 0xffffu, big >> 16);
+                            const float factor = row_divisor(__uint_as_float(most << 16)), inv = 1.f / factor;
+                            factors[row] = factor;
+#pragma unroll 4
+                            for (int c = 0; c < kChunks; ++c) {
+                                const uint32_t at = chunk_at(tile, row & 127, c);
+                                const uint4 v = ld_shared16(at);
                                 const float2 a = Pair<T>::unpack(v.x), b = Pair<T>::unpack(v.y), d = Pair<T>::unpack(v.z),
                                              e = Pair<T>::unpack(v.w);
-                                float amax = fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(b.x), fabsf(b.y))),
-                                                   fmaxf(fmaxf(fabsf(d.x), fabsf(d.y)), fmaxf(fabsf(e.x), fabsf(e.y))));
-#pragma unroll
-                                for (int k = 1; k < kChunks; k <<= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, k));
-                                factor = row_divisor(amax);
-                                const float inv = 1.f / factor;
-                                v.x = Pair<__half>::pack(a.x * inv, a.y * inv);
-                                v.y = Pair<__half>::pack(b.x * inv, b.y * inv);
-                                v.z = Pair<__half>::pack(d.x * inv, d.y * inv);
-                                v.w = Pair<__half>::pack(e.x * inv, e.y * inv);
+                                st_shared16(at, Pair<__half>::pack(a.x * inv, a.y * inv),
+                                            Pair<__half>::pack(b.x * inv, b.y * inv), Pair<__half>::pack(d.x * inv, d.y * inv),
+                                            Pair<__half>::pack(e.x * inv, e.y * inv));
                             }
-                            st_shared16(dst, v.x, v.y, v.z, v.w);
-                            if (c == 0) factors[row] = factor;
                         }
+                    } else if constexpr (Q4) {
+                        for (int s = 0; s < 64; s += 32) factors[64 * w + s + lane] = 1.f;
                     }
-                    if constexpr (!Q4) asm volatile("cp.async.wait_all;" ::: "memory");
                     fence_async_shared();
                     mbar_arrive(&bars->q_full);
                 }
@@ -574,6 +700,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                     const uint32_t bad = *reinterpret_cast<volatile uint32_t*>(&bars->raw_bad[raw.at]);
                     const int t = lane & 3;                         // quarter of a row: D/4 elements
                     constexpr int kWords = D / 32;                  // of codes a lane holds per key
+                    // Every key of the tile is seen by some row and lies in a good page.
+                    const bool all = (bad & 0xff) == 0 && first + kTileKeys - 1 <= last &&
+                                     (it.pos0 - first < p.window || first + kTileKeys - 1 < p.sinks);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int row = 32 * w + 8 * i + (lane >> 2), j = first + row;
@@ -596,8 +725,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                             scale = u;
                         }
                         // Keys that no row sees and bad pages read as zeros, whatever the raw tile holds.
-                        const bool take = !((bad >> (row >> 4)) & 1) && j <= last && (it.pos0 - j < p.window || j < p.sinks);
-                        if (!take) scale = 0;
+                        if (!all && (((bad >> (row >> 4)) & 1) || j > last || (it.pos0 - j >= p.window && j >= p.sinks))) scale = 0;
                         const uint32_t lo = scale & 0xff, hi = D == 128 ? scale >> 8 : lo;
                         const uint32_t s_lo = scales_to_half(lo | (lo << 8)), s_hi = scales_to_half(hi | (hi << 8));
 #pragma unroll
@@ -629,10 +757,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
         const int token = row / p.group;
         const int head = row - token * p.group;
         uint32_t s_phase = 0, q_phase = 0, o_phase = 0;
+        Ring<kWork> work;
         for (int x = blockIdx.x; x < items; x += gridDim.x) {
-            const AttnItem it = tile_item(p, x);
-            if (it.tokens == 0) continue;
-            const KeyTiles kt = key_tiles<kTileKeys>(p, it);
+            AttnItem it;
+            KeyTiles kt;
+            if (!take_work(bars, work, p.status, it, kt)) break;
             const int n = kt.end - kt.begin;
             const bool live = token < it.tokens;
             const int pos = live ? it.pos0 + token : -1;
@@ -651,25 +780,25 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                 if (!(ok = warp_wait(&bars->s_full[i], s_phase, abort, p.status))) break;
                 s_phase ^= 1;
                 tc_fence_after();
+                const int first = kt.first_key<kTileKeys>(kt.begin + j);
+                const bool whole = first + kTileKeys - 1 <= it.pos0 &&
+                                   (last - first < p.window || first + kTileKeys - 1 < p.sinks);
+                // Columns that this row sees: [lo, hi] and those below `head_cols` (sinks).
+                const int hi = pos - first;
+                const int lo = pos - first >= p.window ? pos - first - p.window + 1 : 0;
+                const int head_cols = p.sinks - first;
                 uint32_t sr[kTileKeys];
 #pragma unroll
                 for (int c = 0; c < kTileKeys; c += 32) tmem_load32(s_at + c, sr + c);
                 tc_wait_ld(sr);
 #pragma unroll
                 for (int c = 32; c < kTileKeys; c += 32) after_wait_ld(sr + c);
-                const int first = kt.first_key<kTileKeys>(kt.begin + j);
-                const bool whole = first + kTileKeys - 1 <= it.pos0 &&
-                                   (last - first < p.window || first + kTileKeys - 1 < p.sinks);
                 if (!whole) {
-                    // Visible columns: [lo, hi] and those below `head_cols` (sinks).
-                    const int hi = pos - first;
-                    const int lo = pos - first >= p.window ? pos - first - p.window + 1 : 0;
-                    const int head_cols = p.sinks - first;
 #pragma unroll
                     for (int c = 0; c < kTileKeys; ++c)
                         if (c > hi || (c < lo && c >= head_cols)) sr[c] = __float_as_uint(-INFINITY);
                 }
-                // Four chains of three-way maxima. A NaN among the scores makes the row's result NaN.
+                // Four chains of three-way maxima; NaN where a score is NaN.
                 float best[4] = {top, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int c = 0; c < kTileKeys; c += 8)
@@ -678,26 +807,25 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                         best[k] = max3(best[k], __uint_as_float(sr[c + 2 * k]), __uint_as_float(sr[c + 2 * k + 1]));
                 const float next = max3(max3(best[0], best[1], best[2]), best[3], best[3]);
                 // Keep the old maximum while weights stay below 2^8.
-                const bool grow = j == 0 || !((next - top) * scale <= 8.f);
+                const bool grow = j == 0 || (!(next == top) && !((next - top) * scale <= 8.f));
                 const float old = top;
                 if (grow) top = next;
                 // An infinite score gives NaN, as inf - inf does in the formula.
                 const float ref = top == -INFINITY ? 0.f : top == INFINITY ? NAN : top * scale;
-                if (j > 0 && __any_sync(~0u, grow && next != old)) {
-                    const float shrink = old == -INFINITY ? 0.f : exp2_approx(old * scale - ref);
+                if (j > 0 && __any_sync(~0u, grow)) {
+                    const float shrink = !grow ? 1.f : old == -INFINITY ? 0.f : exp2_approx(old * scale - ref);
                     sum *= shrink;
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 8) {
+                        uint32_t o[8];
+                        tmem_load8(o_at + c, o);
 #pragma unroll
-                    for (int c = 0; c < D; c += 32) {
-                        uint32_t o[32];
-                        tmem_load32(o_at + c, o);
-                        tc_wait_ld(o);
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * shrink);
-                        tmem_store32(o_at + c, o);
+                        for (int k = 0; k < 8; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * shrink);
+                        tmem_store8(o_at + c, o);
                     }
                 }
-                uint64_t part[2] = {0, 0};
                 const uint64_t scale2 = pair2(scale, scale), ref2 = pair2(-ref, -ref);
+                uint64_t part[2] = {0, 0};
 #pragma unroll
                 for (int c = 0; c < kTileKeys; c += 32) {
                     uint32_t w[16];
@@ -725,52 +853,54 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                 mbar_arrive(&bars->p_full[i]);
             }
             if (!ok) break;
+            if (it.tokens == 0) continue;
             if (n > 0) {
                 if (!warp_wait(&bars->o_full[i], o_phase, abort, p.status)) break;
                 o_phase ^= 1;
                 tc_fence_after();
             }
-            // A row that saw no key: sum 0.
+            // A row that saw no key has the sum 0 and gives zeros.
             const float m2 = top == -INFINITY ? 0.f : top * scale;
             const float inv = p.out_scale / sum;
+            const bool none = n <= 0 || sum == 0.f;
             const int64_t at = (static_cast<int64_t>(it.q0 + token) * p.heads + it.head * p.group + head) * p.splits + it.split;
             char* dst = p.out + (it.q0 + token) * p.o_token_stride + (it.head * p.group + head) * p.o_head_stride;
             if (live && p.splits > 1)
                 *reinterpret_cast<float2*>(p.ws_ml + at * 2) = make_float2(top == -INFINITY ? top : m2, sum);
+            bool nan = false;
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
-                float v[32];
+                uint32_t o[32];
                 __syncwarp();
                 if (n > 0) {
-                    uint32_t o[32];
                     tmem_load32(o_at + c, o);
                     tc_wait_ld(o);
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) v[k] = __uint_as_float(o[k]);
                 }
-                if (!live) continue;
-                bool nan = false;
+                if (none) {
 #pragma unroll
-                for (int k = 0; k < 32; ++k) {
-                    if (n <= 0 || sum == 0.f) v[k] = 0.f;
-                    nan |= isnan(v[k]);
+                    for (int k = 0; k < 32; ++k) o[k] = 0;
                 }
-                if (nan && !isnan(sum)) visible_keys_only<T, D, Q4, 32>(p, it, kt, kTileKeys, row, m2, c, v);
-                if (p.splits > 1) {
+                float any = 0.f;                                    // NaN where an element is (0 * infinity too)
 #pragma unroll
-                    for (int k = 0; k < 32; k += 4)
-                        *reinterpret_cast<float4*>(p.ws_o + at * D + c + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                for (int k = 0; k < 32; ++k) any = fmaf(__uint_as_float(o[k]), 0.f, any);
+                nan |= isnan(any);
+                if (!live) {
+                } else if (p.splits > 1) {
+#pragma unroll
+                    for (int k = 0; k < 32; k += 8) store32(p.ws_o + at * D + c + k, o + k, true);
                 } else {
+                    const float f = none ? 0.f : inv;
 #pragma unroll
-                    for (int k = 0; k < 32; k += 8) {
-                        uint32_t o[4];
+                    for (int k = 0; k < 32; k += 16) {
+                        uint32_t h[8];
 #pragma unroll
-                        for (int u = 0; u < 4; ++u)
-                            o[u] = sum == 0.f ? 0u : Pair<T>::pack(v[k + 2 * u] * inv, v[k + 2 * u + 1] * inv);
-                        *reinterpret_cast<uint4*>(dst + (c + k) * 2) = make_uint4(o[0], o[1], o[2], o[3]);
+                        for (int u = 0; u < 8; ++u)
+                            h[u] = Pair<T>::pack(__uint_as_float(o[k + 2 * u]) * f, __uint_as_float(o[k + 2 * u + 1]) * f);
+                        store32(dst + (c + k) * 2, h, p.out_wide);
                     }
                 }
             }
+            if (live && nan && !isnan(sum)) visible_row<T, D, Q4>(p, it, kt, kTileKeys, row, m2, inv, dst, at);
             // O has been read: this thread's next arrival at p_full lets the products write it again.
         }
     }
@@ -828,7 +958,7 @@ static int encode_maps(const AttnParams& p, int head_dim, bool bf16, TileMaps* m
 template <typename T, int D, bool Q4>
 static int run_tile(const AttnParams& p, int device, int sms, cudaStream_t stream) {
     constexpr int smem = TileConfig<D, Q4>::kSmem;
-    static_assert(smem <= 227 * 1024 && sizeof(TileBars<D, Q4>) <= 512, "shared memory of the tile kernel");
+    static_assert(smem <= 227 * 1024 && sizeof(TileBars<D, Q4>) <= 768, "shared memory of the tile kernel");
     static std::atomic<uint64_t> done{0};               // devices that have the opt-in
     const uint64_t bit = 1ull << device;
     if (!(done.load(std::memory_order_relaxed) & bit)) {
