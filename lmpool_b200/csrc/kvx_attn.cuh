@@ -251,30 +251,48 @@ __device__ __forceinline__ float cache_element(const AttnParams& p, const char* 
 // NaN in rows that do not see that key. Such a row (finite sum, NaN in the
 // output) is computed again from its visible keys alone: out[d0 + i], i < N, for
 // the maximum m2 (of scale_log2 * score) that the tiles found. Only inputs that are not finite come here.
-template <typename T, int D, bool Q4, int N>
-__device__ __noinline__ void visible_keys_only(const AttnParams& p, const AttnItem& it, const KeyTiles& kt, int tile_keys,
-                                               int row, float m2, int d0, float* acc) {
+template <typename T, int D, bool Q4, typename F>
+__device__ __forceinline__ void for_visible_keys(const AttnParams& p, const AttnItem& it, const KeyTiles& kt, int tile_keys,
+                                                 int row, F&& each) {
     const int token = row / p.group;
     const int head = it.head * p.group + row % p.group;
     const int pos = it.pos0 + token;
     const T* q = reinterpret_cast<const T*>(p.q + (it.q0 + token) * p.q_token_stride + head * p.q_head_stride);
     const int32_t* table = p.table + it.seq * p.table_stride;
-    for (int i = 0; i < N; ++i) acc[i] = 0.f;
     for (int i = kt.begin; i < kt.end; ++i) {
         const int first = (i < kt.head ? i : i + kt.skip) * tile_keys;
         for (int j = first; j < first + tile_keys; ++j) {
             if (!visible(p, pos, j)) continue;
             const int blk = j / p.block_size, off = j - blk * p.block_size;
             const int64_t page = page_offset(p, table, blk);
-            if (page < 0) continue;
             float s = 0.f;
-            for (int d = 0; d < D; ++d)
-                s = fmaf(static_cast<float>(q[d]), cache_element<T, D, Q4>(p, p.k, page, off, it.head, d), s);
-            const float w = exp2f(fmaf(s, p.scale_log2, -m2));
-            for (int d = 0; d < N; ++d)
-                acc[d] = fmaf(w, cache_element<T, D, Q4>(p, p.v, page, off, it.head, d0 + d), acc[d]);
+            if (page >= 0)
+                for (int d = 0; d < D; ++d)
+                    s = fmaf(static_cast<float>(q[d]), cache_element<T, D, Q4>(p, p.k, page, off, it.head, d), s);
+            each(s, page, off);
         }
     }
+}
+template <typename T, int D, bool Q4, int N>
+__device__ __noinline__ void visible_keys_only(const AttnParams& p, const AttnItem& it, const KeyTiles& kt, int tile_keys,
+                                               int row, float m2, int d0, float* acc) {
+    for (int i = 0; i < N; ++i) acc[i] = 0.f;
+    for_visible_keys<T, D, Q4>(p, it, kt, tile_keys, row, [&](float s, int64_t page, int off) {
+        if (page < 0) return;                       // reads as zeros
+        const float w = exp2f(fmaf(s, p.scale_log2, -m2));
+        for (int d = 0; d < N; ++d)
+            acc[d] = fmaf(w, cache_element<T, D, Q4>(p, p.v, page, off, it.head, d0 + d), acc[d]);
+    });
+}
+// Maximum and sum of such a row.
+template <typename T, int D, bool Q4>
+__device__ __noinline__ void visible_scores(const AttnParams& p, const AttnItem& it, const KeyTiles& kt, int tile_keys, int row,
+                                            float* m2, float* sum) {
+    float m = -INFINITY, l = 0.f;
+    for_visible_keys<T, D, Q4>(p, it, kt, tile_keys, row, [&](float s, int64_t, int) { m = fmaxf(m, s * p.scale_log2); });
+    for_visible_keys<T, D, Q4>(p, it, kt, tile_keys, row, [&](float s, int64_t, int) { l += exp2f(fmaf(s, p.scale_log2, -m)); });
+    *m2 = m;
+    *sum = l;
 }
 
 // ---------------------------------------------------------------------------

@@ -7,17 +7,22 @@
 // one tile's softmax runs under the other's products. Warps:
 //   0-3, 4-7  softmax of row tile 0 and 1: a thread owns a row;
 //   8-11      queries into shared memory; edge tiles of a 16-bit cache; widening of a 4-bit one;
-//   12        one thread issues the products;
+//   12, 15    issue the products of row tile 0 and 1 (two warps, because a wait of one stands in
+//             the queue behind its own products: one warp for both left the tensor cores idle
+//             half of the time);
 //   13        issues the bulk copies;
-//   14        looks up items ahead (lengths, offsets, ranges of keys; 15 idle).
-// Tensor memory (512 columns): S0, S1 (128 fp32 columns each), O0, O1 (D each).
-// The weights P overwrite the first half of their S as 16-bit pairs and are the A
-// operand of O += P V straight from tensor memory. Per row tile i and key tile j the
-// issuing thread runs  O_i += P_i(j) V(j), S_i = Q_i K(j+1)^T  in that order: products
-// of one thread execute in order, so S_i(j+1) cannot overtake the reading of P_i(j), and
-// when its completion reaches the softmax warps, O_i is complete up to j and idle:
-// they may rescale it without a barrier of its own. They do so only when a row's
-// maximum grows by more than 2^8 (weights then stay below 2^8, exact in the sums).
+//   14        looks up items ahead (lengths, offsets, ranges of keys);
+//   16-19     write finished rows while the others are at the next item.
+// Tensor memory (512 columns): per row tile two score buffers of 64 columns (S), then
+// O0, O1 (D each). A step is 64 keys: S_i(u) = Q_i K(u)^T into buffer u % 2; its weights P
+// overwrite the first half of the buffer as 16-bit pairs and are the A operand of O_i +=
+// P_i(u) V(u) straight from tensor memory. The issuing warp runs, per step,
+// O_i += P_i(u) V(u), then S_i(u + 2) into the buffer that this frees: the softmax of step
+// u + 1 has its scores already and never waits for a product of its own. (With one
+// buffer of 128 keys it did, for the 1400 clocks of both products: 3300 clocks per 128 keys.)
+// Products of one thread execute in order, so S_i(u + 2) cannot overtake the reading of P_i(u).
+// A row's maximum may be stale by 2^8 (weights stay below 2^8, exact in the sums); only
+// when it grows by more do the softmax warps rescale O, once O_i += P_i(u - 1) is done.
 //
 // Shared memory holds operand rows of 64 elements (128 bytes) in the 128-byte
 // swizzle: 16-byte chunk c of row r at chunk c ^ (r % 8). Queries and keys are K-major
@@ -51,8 +56,9 @@
 
 namespace kvx {
 
-constexpr int kTileThreads = 512;
+constexpr int kTileThreads = 640;
 constexpr int kTileKeys = 128;
+constexpr int kStepKeys = 64;                  // keys of a step
 constexpr int kHalfRows = 128;                 // rows of one of the two row tiles
 constexpr int kFmaPairs = 3;                   // of 8 pairs of exponentials, on the FMA units
 constexpr uint32_t kMaxWaitPolls = 1u << 22;   // each poll may suspend for a hardware-chosen time
@@ -69,7 +75,8 @@ struct TileConfig {
     static constexpr int kRing = 2 * kTileBytes;                  // after the two query tiles
     static constexpr int kRaw = kRing + kStages * kTileBytes;
     static constexpr int kFactors = kRaw + kRawStages * kRawBytes;
-    static constexpr int kBars = kFactors + 2 * kHalfRows * 4;
+    static constexpr int kSums = kFactors + (Q4 ? 2 * kHalfRows * 4 : 0);
+    static constexpr int kBars = kSums + 2 * kHalfRows * 4;
     static constexpr int kSmem = 1024 + kBars + 768;
 };
 
@@ -139,6 +146,18 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t* r) {
           "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr));
+}
+__device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+        "[%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::
+                       "memory");
 }
 __device__ __forceinline__ void tmem_load8(uint32_t addr, uint32_t* r) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
@@ -233,6 +252,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
+// The n lowest bits; none for n <= 0, all for n >= 32.
+__device__ __forceinline__ uint32_t low_bits(int n) {
+    return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u;
+}
 // 32 bytes of one row: a whole memory sector where the address allows it.
 __device__ __forceinline__ void store32(void* p, const uint32_t* r, bool wide) {
     if (wide) {
@@ -276,14 +299,15 @@ struct TileWork {
     KeyTiles kt;
 };
 constexpr int kWork = 4;       // items looked up ahead
-constexpr int kRoles = 14;     // warps that take each item: 0-13
+constexpr int kRoles = 19;     // warps that take each item: all but 14
 
 template <int D, bool Q4>
 struct TileBars {
     uint64_t full[TileConfig<D, Q4>::kStages], empty[TileConfig<D, Q4>::kStages];
     uint64_t raw_full[4], raw_empty[4];
     uint64_t q_full, q_empty;
-    uint64_t s_full[2], p_full[2], o_full[2];
+    uint64_t s_full[2][2], p_full[2][2];     // [row tile][score buffer]
+    uint64_t pv_done[2], o_full[2], o_free[2], sums_full[2];
     uint64_t drain;
     uint64_t work_full[kWork], work_empty[kWork];
     TileWork work[kWork];
@@ -331,13 +355,19 @@ __device__ __forceinline__ AttnItem tile_item(const AttnParams& p, int x) {
 // Writes a row again from its visible keys alone (see visible_keys_only).
 template <typename T, int D, bool Q4>
 __device__ __noinline__ void visible_row(const AttnParams& p, const AttnItem& it, const KeyTiles& kt, int tile_keys, int row,
-                                         float m2, float inv, char* dst, int64_t at) {
+                                         char* dst, int64_t at) {
+    float m2, sum = 1.f, v[32];
+    if (p.splits > 1) {
+        m2 = p.ws_ml[at * 2];                       // what the other splits are joined with
+        if (m2 == -INFINITY) m2 = 0.f;
+    } else {
+        visible_scores<T, D, Q4>(p, it, kt, tile_keys, row, &m2, &sum);
+    }
     for (int c = 0; c < D; c += 32) {
-        float v[32];
         visible_keys_only<T, D, Q4, 32>(p, it, kt, tile_keys, row, m2, c, v);
         for (int k = 0; k < 32; ++k) {
             if (p.splits > 1) p.ws_o[at * D + c + k] = v[k];
-            else reinterpret_cast<T*>(dst)[c + k] = static_cast<T>(v[k] * inv);
+            else reinterpret_cast<T*>(dst)[c + k] = static_cast<T>(v[k] * (p.out_scale / sum));
         }
     }
 }
@@ -441,6 +471,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
     const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
     char* smem = raw + (base - smem_addr(raw));
     float* factors = reinterpret_cast<float*>(smem + C::kFactors);  // what each query row was divided by
+    float* sums = reinterpret_cast<float*>(smem + C::kSums);        // sums of weights, for warps 16-19
     auto* bars = reinterpret_cast<TileBars<D, Q4>*>(smem + C::kBars);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     griddep_launch_dependents();
@@ -449,20 +480,25 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
         if (lane == 0) {
             for (int i = 0; i < C::kStages; ++i) {
                 mbar_init(&bars->full[i], Q4 ? 128 : 5);    // 16-bit: warps 8-11 and 13
-                mbar_init(&bars->empty[i], 1);
+                mbar_init(&bars->empty[i], 2);
             }
             for (int i = 0; i < 4; ++i) {
                 mbar_init(&bars->raw_full[i], 1);
                 mbar_init(&bars->raw_empty[i], 128);
             }
             mbar_init(&bars->q_full, 128);
-            mbar_init(&bars->q_empty, 1);
+            mbar_init(&bars->q_empty, 2);
             for (int i = 0; i < 2; ++i) {
-                mbar_init(&bars->s_full[i], 1);
-                mbar_init(&bars->p_full[i], 128);
+                for (int h = 0; h < 2; ++h) {
+                    mbar_init(&bars->s_full[i][h], 1);
+                    mbar_init(&bars->p_full[i][h], 128);
+                }
+                mbar_init(&bars->pv_done[i], 1);
                 mbar_init(&bars->o_full[i], 1);
+                mbar_init(&bars->o_free[i], 128);
+                mbar_init(&bars->sums_full[i], 128);
             }
-            mbar_init(&bars->drain, 1);
+            mbar_init(&bars->drain, 2);
             for (int i = 0; i < kWork; ++i) {
                 mbar_init(&bars->work_full[i], 1);
                 mbar_init(&bars->work_empty[i], kRoles);
@@ -475,32 +511,101 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
     __syncthreads();
     tc_fence_after();
     griddep_wait();
-    const uint32_t tmem = bars->tmem;
+    constexpr uint32_t tmem = 0;               // all 512 columns are this CTA's: they start at 0
     uint32_t* abort = &bars->abort;
     const int items = p.tile_slots * p.kv_heads * p.splits;
 
-    // Registers: 4 x 128 a thread at launch, 2 x 208 + 56 + 40 from here on.
-    if (warp >= 12) {
-        give_registers<40>();
-        if (warp == 12) {
-            // ---- products ---- (the whole warp keeps step, so that addresses stay uniform; one lane issues)
-            constexpr uint32_t qk = instruction(std::is_same<M, __nv_bfloat16>::value, false, kTileKeys);
+    // Registers: 5 x 96 a thread at launch; from here on 2 x 128, 72, 56, and 96 for the warps that call functions.
+    if (warp >= 16) {
+        // ---- finished rows ----
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        uint32_t phase = 0;
+        bool ok = true;
+        Ring<kWork> work;
+        for (int x = blockIdx.x; x < items && ok; x += gridDim.x) {
+            AttnItem it;
+            KeyTiles kt;
+            if (!take_work(bars, work, p.status, it, kt)) break;
+            if (it.tokens == 0) continue;
+            const int n = kt.end - kt.begin;
+#pragma unroll 1
+            for (int i = 0; i < 2; ++i) {
+                const int row = (threadIdx.x & 127) + i * kHalfRows;
+                const int token = row / p.group, head = row - token * p.group;
+                const bool live = token < it.tokens;
+                const uint32_t o_at = tmem + lanes + 256 + i * D;
+                float sum = 0.f;
+                if (n > 0) {
+                    if (!(ok = warp_wait(&bars->sums_full[i], phase, abort, p.status))) break;
+                    if (!(ok = warp_wait(&bars->o_full[i], phase, abort, p.status))) break;
+                    tc_fence_after();
+                    sum = sums[row];
+                }
+                // A row that saw no key has the sum 0 and gives zeros.
+                const bool none = sum == 0.f;
+                const float inv = none ? 0.f : p.out_scale / sum;
+                const int64_t at =
+                    (static_cast<int64_t>(it.q0 + token) * p.heads + it.head * p.group + head) * p.splits + it.split;
+                char* dst = p.out + (it.q0 + token) * p.o_token_stride + (it.head * p.group + head) * p.o_head_stride;
+                if (n <= 0 && live && p.splits > 1) *reinterpret_cast<float2*>(p.ws_ml + at * 2) = make_float2(-INFINITY, 0.f);
+                bool nan = false;
+#pragma unroll 1
+                for (int c = 0; c < D; c += 16) {
+                    uint32_t o[16];
+                    __syncwarp();
+                    if (n > 0) tmem_load16(o_at + c, o);
+                    if (none) {
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) o[k] = 0;
+                    }
+                    float any = 0.f;                                // NaN where an element is not finite
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) any = fmaf(__uint_as_float(o[k]), 0.f, any);
+                    nan |= isnan(any);
+                    if (!live) {
+                    } else if (p.splits > 1) {
+                        store32(p.ws_o + at * D + c, o, true);
+                        store32(p.ws_o + at * D + c + 8, o + 8, true);
+                    } else {
+                        uint32_t h[8];
+#pragma unroll
+                        for (int u = 0; u < 8; ++u)
+                            h[u] = Pair<T>::pack(__uint_as_float(o[2 * u]) * inv, __uint_as_float(o[2 * u + 1]) * inv);
+                        store32(dst + c * 2, h, p.out_wide);
+                    }
+                }
+                if (n > 0) {
+                    tc_fence_before();
+                    mbar_arrive(&bars->o_free[i]);
+                }
+                if (live && nan && !isnan(sum)) visible_row<T, D, Q4>(p, it, kt, kTileKeys, row, dst, at);
+            }
+            if (n > 0) phase ^= 1;
+        }
+    } else if (warp >= 12) {
+        give_registers<56>();
+        if (warp == 12 || warp == 15) {
+            // ---- products of one row tile ---- (the whole warp keeps step, one lane issues)
+            const int i = warp == 15;
+            constexpr uint32_t qk = instruction(std::is_same<M, __nv_bfloat16>::value, false, kStepKeys);
             constexpr uint32_t pv = instruction(std::is_same<M, __nv_bfloat16>::value, true, D);
             const bool leader = elect_one();
-            const uint64_t q_desc = operand(base, 16), k_desc = operand(base + C::kRing, 16),
+            const uint64_t q_desc = operand(base + i * C::kTileBytes, 16), k_desc = operand(base + C::kRing, 16),
                            v_desc = operand(base + C::kRing, C::kSlabBytes);
+            const uint32_t s_at = tmem + i * 2 * kStepKeys, o_at = tmem + 256 + i * D;
             Ring<C::kStages> ring;
-            uint32_t q_phase = 0, p_phase = 0;
-            auto scores = [&](int i, int stage) {
+            Ring<kWork> work;
+            uint32_t q_phase = 0, p_phase = 0, free_phase = 1;
+            // Scores against the keys of half h of a stage, into buffer h.
+            auto scores = [&](int h, int stage) {
                 if (leader) {
-                    const uint64_t a = q_desc + i * (C::kTileBytes >> 4), b = k_desc + stage * (C::kTileBytes >> 4);
+                    const uint64_t b = k_desc + stage * (C::kTileBytes >> 4) + h * (kStepKeys * 128 >> 4);
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k) {
-                        constexpr int kPerSlab = 4;
-                        const int off = ((k / kPerSlab) * C::kSlabBytes + (k % kPerSlab) * 32) >> 4;
-                        tc_mma_ss(tmem + i * kTileKeys, a + off, b + off, qk, k > 0);
+                        const int off = ((k / 4) * C::kSlabBytes + (k % 4) * 32) >> 4;
+                        tc_mma_ss(s_at + h * kStepKeys, q_desc + off, b + off, qk, k > 0);
                     }
-                    tc_commit(&bars->s_full[i]);
+                    tc_commit(&bars->s_full[i][h]);
                 }
                 __syncwarp();
             };
@@ -508,7 +613,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                 if (leader) tc_commit(bar);
                 __syncwarp();
             };
-            Ring<kWork> work;
             for (int x = blockIdx.x; x < items; x += gridDim.x) {
                 AttnItem it;
                 KeyTiles kt;
@@ -522,7 +626,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                 scores(0, ring.at);
                 scores(1, ring.at);
                 commit(&bars->empty[ring.at]);
-                if (n == 1) commit(&bars->q_empty);
                 ring.next();
                 bool ok = true;
                 for (int j = 0; j < n && ok; ++j) {
@@ -530,26 +633,27 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                     ring.next();
                     if (!(ok = warp_wait(&bars->full[v.at], v.phase, abort, p.status))) break;
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        if (!(ok = warp_wait(&bars->p_full[i], p_phase, abort, p.status))) break;
+                    for (int h = 0; h < 2; ++h) {
+                        if (!(ok = warp_wait(&bars->p_full[i][h], p_phase, abort, p.status))) break;
+                        if (j == 0 && h == 0 && !(ok = warp_wait(&bars->o_free[i], free_phase, abort, p.status))) break;
                         tc_fence_after();
                         if (leader) {
-                            const uint64_t b = v_desc + v.at * (C::kTileBytes >> 4);
+                            const uint64_t b = v_desc + v.at * (C::kTileBytes >> 4) + h * (kStepKeys * 128 >> 4);
 #pragma unroll
-                            for (int k = 0; k < kTileKeys / 16; ++k)
-                                tc_mma_ts(tmem + 256 + i * D, tmem + i * kTileKeys + k * 8, b + k * (2048 >> 4), pv,
-                                          j > 0 || k > 0);
+                            for (int k = 0; k < kStepKeys / 16; ++k)
+                                tc_mma_ts(o_at, s_at + h * kStepKeys + k * 8, b + k * (2048 >> 4), pv, j > 0 || h > 0 || k > 0);
+                            tc_commit(&bars->pv_done[i]);
                         }
                         __syncwarp();
-                        if (j + 1 < n) {
-                            if (i == 0) {
-                                if (!(ok = warp_wait(&bars->full[ring.at], ring.phase, abort, p.status))) break;
-                                tc_fence_after();
-                            }
-                            scores(i, ring.at);
-                        } else {
-                            commit(&bars->o_full[i]);
+                        if (j + 1 == n) {
+                            if (h == 1) commit(&bars->o_full[i]);
+                            continue;
                         }
+                        if (h == 0) {
+                            if (!(ok = warp_wait(&bars->full[ring.at], ring.phase, abort, p.status))) break;
+                            tc_fence_after();
+                        }
+                        scores(h, ring.at);
                     }
                     if (!ok) break;
                     p_phase ^= 1;
@@ -557,10 +661,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                     if (j + 1 < n) {
                         commit(&bars->empty[ring.at]);
                         ring.next();
-                        if (j + 2 == n) commit(&bars->q_empty);      // no product reads these queries any more
                     }
+                    // No product of this row tile reads these queries any more. (With a single key tile only now, when
+                    // its softmax warps have shown that they are past the item's factors.)
+                    if (j + 2 == n || n == 1) commit(&bars->q_empty);
                 }
                 if (!ok) break;
+                free_phase ^= 1;
             }
             // Nothing of this CTA is in flight when its tensor memory is freed.
             commit(&bars->drain);
@@ -583,7 +690,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
             }
         }
     } else if (warp >= 8) {
-        give_registers<56>();
+        give_registers<72>();
         // ---- queries, edge tiles, widening ----
         const int w = warp - 8;
         Ring<C::kStages> ring;
@@ -748,21 +855,22 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
         }
         if constexpr (!Q4) asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
-        take_registers<208>();
+        take_registers<128>();
         // ---- softmax ----
         const int i = warp >> 2;                                    // row tile
         const int row = (threadIdx.x & 127) + i * kHalfRows;        // row of the item
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t s_at = tmem + lanes + i * kTileKeys, o_at = tmem + lanes + 256 + i * D;
+        const uint32_t s_at = tmem + lanes + i * 2 * kStepKeys, o_at = tmem + lanes + 256 + i * D;
         const int token = row / p.group;
         const int head = row - token * p.group;
-        uint32_t s_phase = 0, q_phase = 0, o_phase = 0;
+        uint32_t s_phase = 0, q_phase = 0, free_phase = 1, pv_phase = 1;
         Ring<kWork> work;
         for (int x = blockIdx.x; x < items; x += gridDim.x) {
             AttnItem it;
             KeyTiles kt;
             if (!take_work(bars, work, p.status, it, kt)) break;
             const int n = kt.end - kt.begin;
+            if (n <= 0) continue;
             const bool live = token < it.tokens;
             const int pos = live ? it.pos0 + token : -1;
             const int last = it.pos0 + it.tokens - 1;
@@ -770,51 +878,56 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
             float scale = p.scale_log2;
             bool ok = true;
             if constexpr (Q4) {
-                if (n > 0) {
-                    if (!warp_wait(&bars->q_full, q_phase, abort, p.status)) break;
-                    q_phase ^= 1;
-                    scale *= factors[row];
-                }
+                if (!warp_wait(&bars->q_full, q_phase, abort, p.status)) break;
+                q_phase ^= 1;
+                scale *= factors[row];
             }
-            for (int j = 0; j < n; ++j) {
-                if (!(ok = warp_wait(&bars->s_full[i], s_phase, abort, p.status))) break;
-                s_phase ^= 1;
+#pragma unroll 1
+            for (int u = 0; u < 2 * n; ++u) {
+                const int h = u & 1;
+                if (!(ok = warp_wait(&bars->s_full[i][h], s_phase, abort, p.status))) break;
+                s_phase ^= h;
                 tc_fence_after();
-                const int first = kt.first_key<kTileKeys>(kt.begin + j);
-                const bool whole = first + kTileKeys - 1 <= it.pos0 &&
-                                   (last - first < p.window || first + kTileKeys - 1 < p.sinks);
-                // Columns that this row sees: [lo, hi] and those below `head_cols` (sinks).
-                const int hi = pos - first;
-                const int lo = pos - first >= p.window ? pos - first - p.window + 1 : 0;
-                const int head_cols = p.sinks - first;
-                uint32_t sr[kTileKeys];
-#pragma unroll
-                for (int c = 0; c < kTileKeys; c += 32) tmem_load32(s_at + c, sr + c);
+                const uint32_t at = s_at + h * kStepKeys;
+                uint32_t sr[kStepKeys];
+                tmem_load32(at, sr);
+                tmem_load32(at + 32, sr + 32);
+                const int first = kt.first_key<kTileKeys>(kt.begin + (u >> 1)) + h * kStepKeys;
+                const bool whole = first + kStepKeys - 1 <= it.pos0 &&
+                                   (last - first < p.window || first + kStepKeys - 1 < p.sinks);
                 tc_wait_ld(sr);
-#pragma unroll
-                for (int c = 32; c < kTileKeys; c += 32) after_wait_ld(sr + c);
+                after_wait_ld(sr + 32);
                 if (!whole) {
+                    // Columns that this row sees, as bits: [lo, hi] and those below `head_cols` (sinks).
+                    const int hi = pos - first;
+                    const int lo = pos - first >= p.window ? pos - first - p.window + 1 : 0;
+                    const int head_cols = p.sinks - first;
 #pragma unroll
-                    for (int c = 0; c < kTileKeys; ++c)
-                        if (c > hi || (c < lo && c >= head_cols)) sr[c] = __float_as_uint(-INFINITY);
+                    for (int b = 0; b < kStepKeys; b += 32) {
+                        const uint32_t seen = low_bits(hi + 1 - b) & (~low_bits(lo - b) | low_bits(head_cols - b));
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) sr[b + c] = seen & (1u << c) ? sr[b + c] : 0xff800000u;
+                    }
                 }
                 // Four chains of three-way maxima; NaN where a score is NaN.
                 float best[4] = {top, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 0; c < kTileKeys; c += 8)
+                for (int c = 0; c < kStepKeys; c += 8)
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         best[k] = max3(best[k], __uint_as_float(sr[c + 2 * k]), __uint_as_float(sr[c + 2 * k + 1]));
                 const float next = max3(max3(best[0], best[1], best[2]), best[3], best[3]);
                 // Keep the old maximum while weights stay below 2^8.
-                const bool grow = j == 0 || (!(next == top) && !((next - top) * scale <= 8.f));
+                const bool grow = u == 0 || (!(next == top) && !((next - top) * scale <= 8.f));
                 const float old = top;
                 if (grow) top = next;
                 // An infinite score gives NaN, as inf - inf does in the formula.
                 const float ref = top == -INFINITY ? 0.f : top == INFINITY ? NAN : top * scale;
-                if (j > 0 && __any_sync(~0u, grow)) {
+                if (u > 0 && __any_sync(~0u, grow)) {
                     const float shrink = !grow ? 1.f : old == -INFINITY ? 0.f : exp2_approx(old * scale - ref);
                     sum *= shrink;
+                    if (!(ok = warp_wait(&bars->pv_done[i], pv_phase, abort, p.status))) break;
+                    tc_fence_after();
 #pragma unroll 1
                     for (int c = 0; c < D; c += 8) {
                         uint32_t o[8];
@@ -827,7 +940,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                 const uint64_t scale2 = pair2(scale, scale), ref2 = pair2(-ref, -ref);
                 uint64_t part[2] = {0, 0};
 #pragma unroll
-                for (int c = 0; c < kTileKeys; c += 32) {
+                for (int c = 0; c < kStepKeys; c += 32) {
                     uint32_t w[16];
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
@@ -844,64 +957,26 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                         const float2 v = unpair(y);
                         w[k] = Pair<M>::pack(v.x, v.y);
                     }
-                    tmem_store16(s_at + c / 2, w);
+                    tmem_store16(at + c / 2, w);
                 }
                 const float2 total = unpair(add2(part[0], part[1]));
                 sum += total.x + total.y;
                 tc_wait_st();
                 tc_fence_before();
-                mbar_arrive(&bars->p_full[i]);
+                mbar_arrive(&bars->p_full[i][h]);
+                pv_phase ^= 1;                                      // of the product that these weights are for
             }
             if (!ok) break;
-            if (it.tokens == 0) continue;
-            if (n > 0) {
-                if (!warp_wait(&bars->o_full[i], o_phase, abort, p.status)) break;
-                o_phase ^= 1;
-                tc_fence_after();
+            if (live && p.splits > 1) {
+                const int64_t at =
+                    (static_cast<int64_t>(it.q0 + token) * p.heads + it.head * p.group + head) * p.splits + it.split;
+                *reinterpret_cast<float2*>(p.ws_ml + at * 2) = make_float2(top == -INFINITY ? top : top * scale, sum);
             }
-            // A row that saw no key has the sum 0 and gives zeros.
-            const float m2 = top == -INFINITY ? 0.f : top * scale;
-            const float inv = p.out_scale / sum;
-            const bool none = n <= 0 || sum == 0.f;
-            const int64_t at = (static_cast<int64_t>(it.q0 + token) * p.heads + it.head * p.group + head) * p.splits + it.split;
-            char* dst = p.out + (it.q0 + token) * p.o_token_stride + (it.head * p.group + head) * p.o_head_stride;
-            if (live && p.splits > 1)
-                *reinterpret_cast<float2*>(p.ws_ml + at * 2) = make_float2(top == -INFINITY ? top : m2, sum);
-            bool nan = false;
-#pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-                uint32_t o[32];
-                __syncwarp();
-                if (n > 0) {
-                    tmem_load32(o_at + c, o);
-                    tc_wait_ld(o);
-                }
-                if (none) {
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) o[k] = 0;
-                }
-                float any = 0.f;                                    // NaN where an element is (0 * infinity too)
-#pragma unroll
-                for (int k = 0; k < 32; ++k) any = fmaf(__uint_as_float(o[k]), 0.f, any);
-                nan |= isnan(any);
-                if (!live) {
-                } else if (p.splits > 1) {
-#pragma unroll
-                    for (int k = 0; k < 32; k += 8) store32(p.ws_o + at * D + c + k, o + k, true);
-                } else {
-                    const float f = none ? 0.f : inv;
-#pragma unroll
-                    for (int k = 0; k < 32; k += 16) {
-                        uint32_t h[8];
-#pragma unroll
-                        for (int u = 0; u < 8; ++u)
-                            h[u] = Pair<T>::pack(__uint_as_float(o[k + 2 * u]) * f, __uint_as_float(o[k + 2 * u + 1]) * f);
-                        store32(dst + (c + k) * 2, h, p.out_wide);
-                    }
-                }
-            }
-            if (live && nan && !isnan(sum)) visible_row<T, D, Q4>(p, it, kt, kTileKeys, row, m2, inv, dst, at);
-            // O has been read: this thread's next arrival at p_full lets the products write it again.
+            // The row's sum goes to warps 16-19 when they are done with the item before.
+            if (!warp_wait(&bars->o_free[i], free_phase, abort, p.status)) break;
+            free_phase ^= 1;
+            sums[row] = sum;
+            mbar_arrive(&bars->sums_full[i]);
         }
     }
     tc_fence_before();
@@ -911,7 +986,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
     // a thousand times what one takes.
     if (*reinterpret_cast<volatile uint32_t*>(abort))
         for (int i = 0; i < 1000; ++i) __nanosleep(1000);
-    if (warp == 12) tmem_free(tmem, 512);
+    if (warp == 12) tmem_free(bars->tmem, 512);
 }
 
 // cuTensorMapEncodeTiled, from the driver that is loaded.
@@ -964,10 +1039,10 @@ static int run_tile(const AttnParams& p, int device, int sms, cudaStream_t strea
     if (!(done.load(std::memory_order_relaxed) & bit)) {
         KVX_CUDA(cudaFuncSetAttribute(attn_tile_kernel<T, D, Q4>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
                  "set attention kernel shared memory");
-        // The roles' register shares add up to what 512 threads of 128 are launched with.
+        // The roles' register shares add up to at most what 640 threads of 96 are launched with.
         cudaFuncAttributes attrs;
         KVX_CUDA(cudaFuncGetAttributes(&attrs, attn_tile_kernel<T, D, Q4>), "query attention kernel");
-        if (attrs.numRegs != 128) return fail(KVX_EUNSUPPORTED, "attention kernel was built with %d registers", attrs.numRegs);
+        if (attrs.numRegs != 96) return fail(KVX_EUNSUPPORTED, "attention kernel was built with %d registers", attrs.numRegs);
         done.fetch_or(bit, std::memory_order_relaxed);
     }
     const int64_t items = static_cast<int64_t>(p.tile_slots) * p.kv_heads * p.splits;
