@@ -11,7 +11,8 @@
 
 namespace kvx {
 
-constexpr int kMaxSplits = 64;
+constexpr int kWaves = 4;
+constexpr int kMinKeys = 512;
 constexpr int kFewRows = 32;            // rows of an item of the split kernel, at most
 constexpr int kTileRows = 256;          // rows of an item of the tile kernel
 
@@ -80,9 +81,10 @@ static AttnPlan plan_of(const kvx_attention* a, int sms) {
     } else {
         pl.nt = avg * group <= 8 ? 1 : avg * group <= 16 ? 2 : 4;
         pl.tile_tokens = a->cu_seqlens_q ? std::max(1, 8 * pl.nt / group) : 1;
-        keys_per_tile = 64;
-        fill = sms * (a->cache_bits == 4 ? 4 : 2);
-        min_tiles = 2;
+        const bool q4 = a->cache_bits == 4;
+        keys_per_tile = q4 && pl.nt < 4 ? 128 : 64;
+        fill = sms * (q4 ? (pl.nt == 1 ? 4 : pl.nt == 2 ? 3 : 2) : 2) * kWaves;
+        min_tiles = kMinKeys / keys_per_tile;
     }
     pl.tile_slots = static_cast<int>(a->cu_seqlens_q ? tokens / pl.tile_tokens + a->num_seqs : a->num_seqs);
     const int64_t items = std::max<int64_t>(seqs, (tokens + pl.tile_tokens - 1) / pl.tile_tokens) * a->num_kv_heads;

@@ -18,6 +18,8 @@
 
 namespace kvx {
 
+constexpr int kMaxSplits = 64;
+
 struct AttnParams {
     const char* q;
     char* out;

@@ -12,11 +12,13 @@
 // 16-bit cache: each warp has a ring of kStages slices (16 keys of K and V) in
 // shared memory, filled by 16-byte cp.async (any page size, any strides; keys
 // that no row sees are filled with zeros), read back by ldmatrix.
-// 4-bit cache: the fragments' order along head_dim is free as long as both
-// operands agree, so a lane loads the codes it multiplies straight from global
-// memory into registers (64 contiguous bytes per key, one slice ahead), turns
-// them into fp16 and scales them there, exactly. Queries go to fp16 too, each row
-// first divided by the power of two below its largest element.
+// 4-bit cache: the ring holds raw slices (16 keys: 1 KiB of codes and 128 bytes of scales of K
+// and of V at head_dim 128, each contiguous in a page), which lanes widen to fp16 and scale on
+// their way into the products, exactly. The fragments' order along head_dim and along the keys
+// is free as long as both operands agree, so a lane takes the codes that lie together: the
+// conversions, four instructions for eight elements with the scaling, bound this path, not
+// the bytes. Queries go to fp16 too, each row first divided by the power of two below its
+// largest element.
 // Weights: for a bf16 cache they are split in two bf16 numbers (2^-17 relative;
 // the tensor cores have time to spare here), for fp16 and 4-bit rounded to fp16.
 
@@ -31,7 +33,8 @@
 namespace kvx {
 
 constexpr int kSplitWarps = 4;
-constexpr int kSplitKeys = 16 * kSplitWarps;   // keys of a tile
+constexpr int kQ4Slices = 2;
+constexpr int kQ4Stages = 2;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
     const int n = take ? 16 : 0;
@@ -76,30 +79,46 @@ __device__ __forceinline__ void mma16816<__half>(float c[4], const uint32_t a[4]
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <int D, bool Q4>
-struct SplitConfig {
-    static constexpr int kStages = 3;
-    static constexpr int kSliceBytes = 2 * 16 * D * 2;                       // K and V of 16 keys
-    static constexpr int kRing = Q4 ? 0 : kStages * kSliceBytes * kSplitWarps;
-    static constexpr int merge_bytes(int rows) { return kSplitWarps * rows * (D + 4) * 4; }
-    static constexpr int smem(int rows) { return kRing > merge_bytes(rows) ? kRing : merge_bytes(rows); }
-};
+template <int N>
+__device__ __forceinline__ void ld_shared(uint32_t (&r)[N], uint32_t addr) {
+    if constexpr (N == 4)
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+    else if constexpr (N == 2)
+        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
+    else
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r[0]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t ld_shared_u16(uint32_t addr) {
+    uint32_t r;
+    asm volatile("{\n\t.reg .u16 t;\n\tld.shared.u16 t, [%1];\n\tcvt.u32.u16 %0, t;\n\t}" : "=r"(r) : "r"(addr) : "memory");
+    return r;
+}
+__device__ __forceinline__ uint32_t ld_shared_u8(uint32_t addr) {
+    uint32_t r;
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(r) : "r"(addr) : "memory");
+    return r;
+}
 
-// A slice of the 4-bit cache as a lane holds it.
-template <int D>
-struct Q4Slice {
-    uint32_t k[2][D / 32];     // keys g and g + 8: codes of d = (D/4) t ...
-    uint32_t ks[2];            // their scales, one byte per 16 elements
-    uint32_t v[4][D / 64];     // keys 2t, 2t+1, 2t+8, 2t+9: codes of d = (D/8) g ...
-    uint32_t vs[2];            // scales of keys (2t, 2t+1) and (2t+8, 2t+9), two bytes each
+template <int D, int NT, bool Q4>
+struct SplitConfig {
+    static constexpr int kSlices = Q4 && NT < 4 ? kQ4Slices : 1;             // slices of 16 keys a warp takes at once
+    static constexpr int kWarpKeys = 16 * kSlices;
+    static constexpr int kKeys = kWarpKeys * kSplitWarps;                    // keys of a tile
+    static constexpr int kStages = Q4 ? kQ4Stages : 3;
+    static constexpr int kCodes = 16 * D / 2, kScales = 16 * D / 16;         // bytes of a 4-bit slice, K or V
+    static constexpr int kStageBytes = Q4 ? kSlices * 2 * (kCodes + kScales) : 2 * 16 * D * 2;
+    static constexpr int kRing = kStages * kStageBytes * kSplitWarps;
+    static constexpr int kMerge = kSplitWarps * 8 * NT * (D + 4) * 4;
+    static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
 };
 
 template <typename T, int D, int NT, bool Q4>
-__global__ void __launch_bounds__(kSplitWarps * 32) attn_split_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(kSplitWarps * 32, Q4 && NT == 1 ? 4 : 2) attn_split_kernel(const __grid_constant__ AttnParams p) {
     using M = typename std::conditional<Q4, __half, T>::type;     // type of the products' operands
-    using C = SplitConfig<D, Q4>;
+    using C = SplitConfig<D, NT, Q4>;
     constexpr int kRows = 8 * NT;
     constexpr int KS = D / 16;                                     // k steps of Q K^T, m tiles of V^T P^T
+    constexpr int NS = C::kSlices;
     constexpr bool kTwoWeights = !Q4 && std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ __align__(128) char smem[];
     griddep_launch_dependents();
@@ -111,10 +130,136 @@ __global__ void __launch_bounds__(kSplitWarps * 32) attn_split_kernel(const __gr
     it.head = blockIdx.y;
     it.split = blockIdx.z;
     if (it.tokens == 0) return;
-    const KeyTiles kt = key_tiles<kSplitKeys>(p, it);
+    const KeyTiles kt = key_tiles<C::kKeys>(p, it);
     const int rows = it.tokens * p.group;
     const int32_t* table = p.table + it.seq * p.table_stride;
     const int last = it.pos0 + it.tokens - 1;
+    const int64_t head_off = it.head * p.head_stride;
+    [[maybe_unused]] const char* k_head = p.k + head_off;
+    [[maybe_unused]] const char* v_head = p.v + head_off;
+
+    // Whether any row of the item sees key j: what no row sees counts nowhere.
+    auto wanted = [&](int j) { return j <= last && (it.pos0 - j < p.window || j < p.sinks); };
+    // Whether a slice of 16 keys holds such a key; whether all of them are.
+    auto touched = [&](int first) { return first <= last && (it.pos0 - (first + 15) < p.window || first < p.sinks); };
+    auto filled = [&](int first) { return first + 15 <= last && (it.pos0 - first < p.window || first + 15 < p.sinks); };
+    auto first_of = [&](int i, int sub) { return kt.template first_key<C::kKeys>(i) + warp * C::kWarpKeys + 16 * sub; };
+
+    // Where this warp's slices lie, for pages that hold whole slices: a lane looks up one of the next 32
+    // slices, a batch ahead, so that no load of keys waits for a table entry.
+    const bool paged16 = p.block_size % 16 == 0;
+    int64_t run_now = -1, run_next = -1;                           // bytes from the head's first key in page 0
+    int gap_now = 0, gap_next = 0;                                 // 4-bit: from the slice's codes to its scales
+    auto look_up = [&](int batch) {
+        const int m = batch * 32 + lane, i = kt.begin + m / NS;
+        run_next = -1;
+        if (i < kt.end) {
+            const int first = first_of(i, m % NS);
+            if (touched(first)) {
+                const int blk = block_of(p, first), in = first - blk * p.block_size;
+                run_next = page_offset(p, table, blk);
+                if (run_next >= 0) run_next += in * (Q4 ? D / 2 : p.slot_stride);
+                gap_next = p.block_size * (D / 2) - in * (D / 2 - D / 16);
+            }
+        }
+    };
+    auto advance = [&](int n) {                                    // before the slices of iteration n are read
+        if ((n * NS) % 32 == 0) {
+            run_now = run_next;
+            gap_now = gap_next;
+            look_up(n * NS / 32 + 1);
+        }
+    };
+    const int count = kt.end - kt.begin;
+    if (paged16) look_up(0);
+
+    // 16-bit cache: slice n of this warp into a stage of its ring.
+    [[maybe_unused]] const uint32_t ring = smem_addr(smem) + warp * C::kStages * C::kStageBytes;
+    [[maybe_unused]] auto fetch16 = [&](int n, int stage) {
+        if (n < count) {
+            constexpr int kChunks = D / 8;                         // 16-byte chunks of a row
+            constexpr int kRowsPerStep = 32 / kChunks;
+            const int first = first_of(kt.begin + n, 0);
+            const int c = lane % kChunks, r_lane = lane / kChunks;
+            const uint32_t dst = ring + stage * C::kStageBytes;
+            int64_t off = -1;                                      // of this lane's row
+            bool all = false;
+            if (paged16) {
+                advance(n);
+                const int64_t run = __shfl_sync(~0u, run_now, n & 31);
+                all = filled(first) && run >= 0;
+                off = run < 0 ? -1 : run + head_off + r_lane * p.slot_stride;
+            } else {
+                const int j = first + (lane & 15);
+                if (wanted(j)) {
+                    const int blk = block_of(p, j);
+                    off = page_offset(p, table, blk);
+                    if (off >= 0) off += (j - blk * p.block_size) * p.slot_stride + head_off;
+                }
+            }
+            if (all) {
+                const char* k_src = p.k + off + 16 * c;
+                const char* v_src = p.v + off + 16 * c;
+#pragma unroll
+                for (int r0 = 0; r0 < 16; r0 += kRowsPerStep) {
+                    const int r = r0 + r_lane;
+                    const uint32_t to = dst + r * (D * 2) + ((c ^ (r & 7)) << 4);
+                    cp_async16(to, k_src + r0 * p.slot_stride, true);
+                    cp_async16(to + 16 * D * 2, v_src + r0 * p.slot_stride, true);
+                }
+            } else {
+                // Zeros for keys that no row sees and for bad pages.
+#pragma unroll
+                for (int r0 = 0; r0 < 16; r0 += kRowsPerStep) {
+                    const int r = r0 + r_lane;
+                    int64_t a = paged16 ? off + r0 * p.slot_stride : __shfl_sync(~0u, off, r);
+                    if (paged16 && (off < 0 || !wanted(first + r))) a = -1;
+                    const int64_t from = (a < 0 ? 0 : a) + c * 16;
+                    const uint32_t to = dst + r * (D * 2) + ((c ^ (r & 7)) << 4);
+                    cp_async16(to, p.k + from, a >= 0);
+                    cp_async16(to + 16 * D * 2, p.v + from, a >= 0);
+                }
+            }
+        }
+        cp_async_commit();
+    };
+    // 4-bit cache: the slices of iteration n into a stage. block_size is a multiple of 16. Keys are
+    // rows of the products in the order 0 4 1 5 2 6 3 7 (and 8 further): a lane's four keys
+    // of V are then t, t + 4, t + 8 and t + 12, rows side by side. Key k of K stands at the
+    // row it is; V's 16-byte chunks are crossed in every second pair of rows, against bank conflicts.
+    constexpr int kRowChunks = D / 32;                             // 16-byte chunks of a row of codes
+    [[maybe_unused]] auto fetch4 = [&](int n, int stage) {
+        if (n < count) {
+            advance(n);
+#pragma unroll
+            for (int z = 0; z < NS; ++z) {
+                const int64_t run = __shfl_sync(~0u, run_now, (n * NS + z) & 31);
+                const int gap = __shfl_sync(~0u, gap_now, (n * NS + z) & 31);
+                const bool take = run >= 0;                        // else nothing to see or a bad page: zeros
+                const char* k_from = k_head + (take ? run : 0);
+                const char* v_from = v_head + (take ? run : 0);
+                const uint32_t dst = ring + stage * C::kStageBytes + z * 2 * (C::kCodes + C::kScales);
+#pragma unroll
+                for (int h = 0; h < C::kCodes / 512; ++h) {
+                    const int chunk = lane + 32 * h, key = chunk / kRowChunks, c = chunk % kRowChunks;
+                    const int k_row = (key & 8) | ((key & 3) << 1) | ((key >> 2) & 1);
+                    cp_async16(dst + k_row * (D / 2) + c * 16, k_from + chunk * 16, take);
+                    cp_async16(dst + C::kCodes + key * (D / 2) + (c ^ (D == 128 ? key & 2 : 0)) * 16, v_from + chunk * 16, take);
+                }
+                constexpr int kScaleChunks = C::kScales / 16;
+                if (lane < 2 * kScaleChunks)
+                    cp_async16(dst + 2 * C::kCodes + lane * 16,
+                               (lane < kScaleChunks ? k_from : v_from) + gap + (lane % kScaleChunks) * 16, take);
+            }
+        }
+        cp_async_commit();
+    };
+    // The first keys are on their way while the queries are read.
+#pragma unroll
+    for (int n = 0; n < C::kStages - 1; ++n) {
+        if constexpr (Q4) fetch4(n, n);
+        else fetch16(n, n);
+    }
 
     // Rows of this lane: n = g of each n tile as B operand, 2t and 2t + 1 as columns of the results.
     uint32_t qf[NT][KS][2];
@@ -184,220 +329,189 @@ __global__ void __launch_bounds__(kSplitWarps * 32) attn_split_kernel(const __gr
         for (int m = 0; m < KS; ++m) o[m][nt][0] = o[m][nt][1] = o[m][nt][2] = o[m][nt][3] = 0.f;
     }
 
-    // One slice: S^T, the softmax step and O^T, given the fragments of K and V.
+    const int key_of_row = Q4 ? (g >> 1) | ((g & 1) << 2) : g;     // the key in row g of S^T
+    // NS slices: S^T, the softmax step and O^T, given the fragments of K and V.
     auto attend = [&](int first, auto&& k_frag, auto&& v_frag) {
-        float s[NT][4];
+        float s[NS][NT][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+        for (int z = 0; z < NS; ++z) {
 #pragma unroll
-        for (int i = 0; i < KS; ++i) {
-            uint32_t a[4];
-            k_frag(i, a);
+            for (int nt = 0; nt < NT; ++nt) s[z][nt][0] = s[z][nt][1] = s[z][nt][2] = s[z][nt][3] = 0.f;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma16816<M>(s[nt], a, qf[nt][i][0], qf[nt][i][1]);
+            for (int i = 0; i < KS; ++i) {
+                uint32_t a[4];
+                k_frag(z, i, a);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma16816<M>(s[z][nt], a, qf[nt][i][0], qf[nt][i][1]);
+            }
         }
         // Every key visible to every row: nothing to mask. (it.pos0 is the oldest row's position.)
-        const bool whole = first + 15 <= it.pos0 && (last - first < p.window || first + 15 < p.sinks);
-        uint32_t pw[NT][2];
-        [[maybe_unused]] uint32_t pl[NT][2];
+        const int end = first + 16 * NS - 1;
+        const bool whole = end <= it.pos0 && (last - first < p.window || end < p.sinks);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+        for (int z = 0; z < NS; ++z)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[z][nt][e] *= row_scale[nt][e & 1];
+        if (!whole) {
+#pragma unroll
+            for (int z = 0; z < NS; ++z)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (!visible(p, pos[nt][e & 1], first + 16 * z + 8 * (e >> 1) + key_of_row)) s[z][nt][e] = -INFINITY;
+        }
+        float top[NT][2];
+        bool grow = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                float x0 = s[nt][c] * row_scale[nt][c], x1 = s[nt][c + 2] * row_scale[nt][c];
-                if (!whole) {
-                    if (!visible(p, pos[nt][c], first + g)) x0 = -INFINITY;
-                    if (!visible(p, pos[nt][c], first + g + 8)) x1 = -INFINITY;
-                }
-                float top = fmaxf(x0, x1);
-                top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
-                top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
-                top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
-                const float next = fmaxf(mx[nt][c], top);
-                const float base = next == -INFINITY ? 0.f : next;
-                const float shrink = exp2_approx(mx[nt][c] - base);
-                mx[nt][c] = next;
-                s[nt][c] = exp2_approx(x0 - base);
-                s[nt][c + 2] = exp2_approx(x1 - base);
-                sum[nt][c] = fmaf(sum[nt][c], shrink, s[nt][c] + s[nt][c + 2]);
+                top[nt][c] = fmaxf(s[0][nt][c], s[0][nt][c + 2]);
 #pragma unroll
-                for (int m = 0; m < KS; ++m) {
-                    o[m][nt][c] *= shrink;
-                    o[m][nt][c + 2] *= shrink;
-                }
+                for (int z = 1; z < NS; ++z) top[nt][c] = fmaxf(top[nt][c], fmaxf(s[z][nt][c], s[z][nt][c + 2]));
+                top[nt][c] = fmaxf(top[nt][c], __shfl_xor_sync(~0u, top[nt][c], 4));
+                top[nt][c] = fmaxf(top[nt][c], __shfl_xor_sync(~0u, top[nt][c], 8));
+                top[nt][c] = fmaxf(top[nt][c], __shfl_xor_sync(~0u, top[nt][c], 16));
+                grow |= top[nt][c] > mx[nt][c] + 8.f;              // also from no key to a first one
             }
+        // Rescale only when a row's maximum grows by more than 2^8: until then weights stay below that.
+        if (__any_sync(~0u, grow)) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint32_t w = Pair<M>::pack(s[nt][2 * h], s[nt][2 * h + 1]);
-                if constexpr (kTwoWeights) {
-                    const float2 r = Pair<M>::unpack(w);
-                    pl[nt][h] = transpose8x8(Pair<M>::pack(s[nt][2 * h] - r.x, s[nt][2 * h + 1] - r.y));
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const float next = fmaxf(mx[nt][c], top[nt][c]);
+                    const float shrink = exp2_approx(mx[nt][c] - (next == -INFINITY ? 0.f : next));
+                    mx[nt][c] = next;
+                    sum[nt][c] *= shrink;
+#pragma unroll
+                    for (int m = 0; m < KS; ++m) {
+                        o[m][nt][c] *= shrink;
+                        o[m][nt][c + 2] *= shrink;
+                    }
                 }
-                pw[nt][h] = transpose8x8(w);
-            }
         }
 #pragma unroll
-        for (int m = 0; m < KS; ++m) {
-            uint32_t a[4];
-            v_frag(m, a);
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                mma16816<M>(o[m][nt], a, pw[nt][0], pw[nt][1]);
-                if constexpr (kTwoWeights) mma16816<M>(o[m][nt], a, pl[nt][0], pl[nt][1]);
+            for (int c = 0; c < 2; ++c) {
+                const float base = mx[nt][c] == -INFINITY ? 0.f : mx[nt][c];
+#pragma unroll
+                for (int z = 0; z < NS; ++z) {
+                    s[z][nt][c] = exp2_approx(s[z][nt][c] - base);
+                    s[z][nt][c + 2] = exp2_approx(s[z][nt][c + 2] - base);
+                    sum[nt][c] += s[z][nt][c] + s[z][nt][c + 2];
+                }
+            }
+#pragma unroll
+        for (int z = 0; z < NS; ++z) {
+            uint32_t pw[NT][2];
+            [[maybe_unused]] uint32_t pl[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t w = Pair<M>::pack(s[z][nt][2 * h], s[z][nt][2 * h + 1]);
+                    if constexpr (kTwoWeights) {
+                        const float2 r = Pair<M>::unpack(w);
+                        pl[nt][h] = transpose8x8(Pair<M>::pack(s[z][nt][2 * h] - r.x, s[z][nt][2 * h + 1] - r.y));
+                    }
+                    pw[nt][h] = transpose8x8(w);
+                }
+#pragma unroll
+            for (int m = 0; m < KS; ++m) {
+                uint32_t a[4];
+                v_frag(z, m, a);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    mma16816<M>(o[m][nt], a, pw[nt][0], pw[nt][1]);
+                    if constexpr (kTwoWeights) mma16816<M>(o[m][nt], a, pl[nt][0], pl[nt][1]);
+                }
             }
         }
-    };
-    // Whether any row of the item sees key j: what no row sees is never read.
-    auto wanted = [&](int j) {
-        return j <= last && (it.pos0 - j < p.window || j < p.sinks);
-    };
-    // Whether a slice of 16 keys holds such a key.
-    auto touched = [&](int first) {
-        return first <= last && (it.pos0 - (first + 15) < p.window || first < p.sinks);
     };
 
-    if constexpr (!Q4) {
-        const uint32_t ring = smem_addr(smem) + warp * C::kStages * C::kSliceBytes;
-        const int64_t head_off = it.head * p.head_stride;
-        constexpr int kChunks = D / 8;                  // 16-byte chunks of a row
-        constexpr int kRowsPerStep = 32 / kChunks;
-        auto fetch = [&](int i, int stage) {
-            if (i < kt.end) {
-                const int first = kt.first_key<kSplitKeys>(i) + 16 * warp;
-                int64_t off = -1;
-                const int j = first + (lane & 15);
-                if (wanted(j)) {
-                    const int blk = block_of(p, j);
-                    off = page_offset(p, table, blk);
-                    if (off >= 0) off += (j - blk * p.block_size) * p.slot_stride + head_off;
-                }
-                const uint32_t dst = ring + stage * C::kSliceBytes;
-                const int c = lane % kChunks;
-#pragma unroll
-                for (int r0 = 0; r0 < 16; r0 += kRowsPerStep) {
-                    const int r = r0 + lane / kChunks;
-                    const int64_t a = __shfl_sync(~0u, off, r);
-                    const int64_t from = (a < 0 ? 0 : a) + c * 16;
-                    const uint32_t to = dst + r * (D * 2) + ((c ^ (r & 7)) << 4);
-                    cp_async16(to, p.k + from, a >= 0);
-                    cp_async16(to + 16 * D * 2, p.v + from, a >= 0);
-                }
-            }
-            cp_async_commit();
-        };
-#pragma unroll
-        for (int i = 0; i < C::kStages - 1; ++i) fetch(kt.begin + i, i);
-        int stage = 0;
-        for (int i = kt.begin; i < kt.end; ++i) {
-            cp_async_wait<C::kStages - 2>();
-            __syncwarp();
-            const int ahead = stage + C::kStages - 1;
-            fetch(i + C::kStages - 1, ahead >= C::kStages ? ahead - C::kStages : ahead);
-            const int first = kt.first_key<kSplitKeys>(i) + 16 * warp;
-            const uint32_t k_at = ring + stage * C::kSliceBytes, v_at = k_at + 16 * D * 2;
+    int stage = 0;
+    for (int n = 0; n < count; ++n) {
+        cp_async_wait<C::kStages - 2>();
+        __syncwarp();
+        const int next = stage + C::kStages - 1;
+        if constexpr (Q4) fetch4(n + C::kStages - 1, next >= C::kStages ? next - C::kStages : next);
+        else fetch16(n + C::kStages - 1, next >= C::kStages ? next - C::kStages : next);
+        const int first = first_of(kt.begin + n, 0);
+        const uint32_t at = ring + stage * C::kStageBytes;
+        if constexpr (!Q4) {
+            const uint32_t v_at = at + 16 * D * 2;
             if (touched(first))
                 attend(
                     first,
-                    [&](int ks, uint32_t a[4]) {
+                    [&](int, int ks, uint32_t a[4]) {
                         const int r = lane & 15, c = 2 * ks + (lane >> 4);
-                        ldmatrix4(a, k_at + r * (D * 2) + ((c ^ (r & 7)) << 4));
+                        ldmatrix4(a, at + r * (D * 2) + ((c ^ (r & 7)) << 4));
                     },
-                    [&](int m, uint32_t a[4]) {
+                    [&](int, int m, uint32_t a[4]) {
                         const int r = (lane & 7) + ((lane >> 4) << 3), c = 2 * m + ((lane >> 3) & 1);
                         ldmatrix4_t(a, v_at + r * (D * 2) + ((c ^ (r & 7)) << 4));
                     });
-            __syncwarp();
-            stage = stage + 1 == C::kStages ? 0 : stage + 1;
-        }
-        cp_async_wait<0>();
-    } else {
-        const int64_t head_off = it.head * p.head_stride;
-        const int scales_at = p.block_size * (D / 2);
-        auto fetch = [&](int i, Q4Slice<D>& x) {
-            x.ks[0] = x.ks[1] = x.vs[0] = x.vs[1] = 0;
+        } else {
+            bool any = false;
 #pragma unroll
-            for (int w = 0; w < D / 32; ++w) x.k[0][w] = x.k[1][w] = 0;
-#pragma unroll
-            for (int w = 0; w < D / 64; ++w) x.v[0][w] = x.v[1][w] = x.v[2][w] = x.v[3][w] = 0;
-            if (i >= kt.end) return;
-            const int first = kt.first_key<kSplitKeys>(i) + 16 * warp;
-            if (!touched(first)) return;
-            // block_size is a multiple of 16: a slice lies in one page.
-            const int blk = block_of(p, first);
-            const int64_t page = page_offset(p, table, blk);
-            if (page < 0) return;
-            const int off = first - blk * p.block_size;
-            const char* kb = p.k + page + head_off;
-            const char* vb = p.v + page + head_off;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int key = g + 8 * h;
-                if (!wanted(first + key)) continue;
-                const char* c = kb + (off + key) * (D / 2) + t * (D / 8);
-                const char* s = kb + scales_at + (off + key) * (D / 16);
-                if constexpr (D == 128) {
-                    const uint4 w = __ldg(reinterpret_cast<const uint4*>(c));
-                    x.k[h][0] = w.x, x.k[h][1] = w.y, x.k[h][2] = w.z, x.k[h][3] = w.w;
-                    x.ks[h] = __ldg(reinterpret_cast<const uint16_t*>(s) + t);
-                } else {
-                    const uint2 w = __ldg(reinterpret_cast<const uint2*>(c));
-                    x.k[h][0] = w.x, x.k[h][1] = w.y;
-                    x.ks[h] = __ldg(reinterpret_cast<const uint8_t*>(s) + t);
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int key = 2 * t + (u & 1) + 8 * (u >> 1);
-                if (!wanted(first + key)) continue;
-                const char* c = vb + (off + key) * (D / 2) + g * (D / 16);
-                const char* s = vb + scales_at + (off + key) * (D / 16);
-                if constexpr (D == 128) {
-                    const uint2 w = __ldg(reinterpret_cast<const uint2*>(c));
-                    x.v[u][0] = w.x, x.v[u][1] = w.y;
-                    x.vs[u >> 1] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const uint8_t*>(s) + g)) << (8 * (u & 1));
-                } else {
-                    x.v[u][0] = __ldg(reinterpret_cast<const uint32_t*>(c));
-                    x.vs[u >> 1] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const uint8_t*>(s) + g / 2)) << (8 * (u & 1));
-                }
-            }
-        };
-        Q4Slice<D> now, ahead;
-        fetch(kt.begin, now);
-        for (int i = kt.begin; i < kt.end; ++i) {
-            fetch(i + 1, ahead);
-            const int first = kt.first_key<kSplitKeys>(i) + 16 * warp;
-            if (touched(first)) {
-                // A lane's scales: D = 128: bytes 2t, 2t + 1 (k steps 0-3, 4-7); D = 64: byte t.
-                uint32_t sc[2][2];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t lo = now.ks[h] & 0xff, hi = D == 128 ? now.ks[h] >> 8 : lo;
-                    sc[h][0] = scales_to_half(lo | (lo << 8));
-                    sc[h][1] = scales_to_half(hi | (hi << 8));
-                }
-                uint32_t kd[2][4];
-                const uint32_t vsc[2] = {scales_to_half(now.vs[0]), scales_to_half(now.vs[1])};
-                uint32_t vd[4][4];
+            for (int z = 0; z < NS; ++z) any |= touched(first + 16 * z);
+            if (any) {
+                uint32_t kc[2][D / 32], sc[2][2], kd[2][4], vc[4][D / 64], vsc[2], vd[4][4];
                 attend(
                     first,
-                    [&](int ks, uint32_t a[4]) {
-                        if ((ks & 1) == 0) {
-                            codes_to_half(now.k[0][ks / 2], kd[0]);
-                            codes_to_half(now.k[1][ks / 2], kd[1]);
+                    [&](int z, int ks, uint32_t a[4]) {
+                        // d = (D/4) t + 4 ks ... of the keys in rows g and g + 8; scale bytes: D = 128: 2t, 2t + 1
+                        // (k steps 0-3, 4-7); D = 64: t.
+                        if (ks == 0) {
+                            const uint32_t from = at + z * 2 * (C::kCodes + C::kScales);
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                ld_shared<D / 32>(kc[h], from + (g + 8 * h) * (D / 2) + t * (D / 8));
+                                const uint32_t s = from + 2 * C::kCodes + (key_of_row + 8 * h) * (D / 16) + t * (D / 64);
+                                const uint32_t both = D == 128 ? ld_shared_u16(s) : ld_shared_u8(s);
+                                sc[h][0] = scales_to_half(__byte_perm(both, 0, 0x0000));
+                                sc[h][1] = D == 128 ? scales_to_half(__byte_perm(both, 0, 0x1111)) : sc[h][0];
+                            }
                         }
-                        const int b = 2 * (ks & 1), z = D == 128 ? ks / 4 : 0;
-                        a[0] = mul_half2(kd[0][b], sc[0][z]);
-                        a[1] = mul_half2(kd[1][b], sc[1][z]);
-                        a[2] = mul_half2(kd[0][b + 1], sc[0][z]);
-                        a[3] = mul_half2(kd[1][b + 1], sc[1][z]);
+                        if ((ks & 1) == 0) {
+                            codes_to_half(kc[0][ks / 2], kd[0]);
+                            codes_to_half(kc[1][ks / 2], kd[1]);
+                        }
+                        const int b = 2 * (ks & 1), y = D == 128 ? ks / 4 : 0;
+                        a[0] = mul_half2(kd[0][b], sc[0][y]);
+                        a[1] = mul_half2(kd[1][b], sc[1][y]);
+                        a[2] = mul_half2(kd[0][b + 1], sc[0][y]);
+                        a[3] = mul_half2(kd[1][b + 1], sc[1][y]);
                     },
-                    [&](int m, uint32_t a[4]) {
+                    [&](int z, int m, uint32_t a[4]) {
                         // Byte m of a key's chunk holds d = (D/8) g + 2m (row g) and + 1 (row g + 8);
-                        // pair the low and the high halves of two neighbouring keys.
+                        // pair the low and the high halves of two keys.
+                        if (m == 0) {
+                            const uint32_t from = at + z * 2 * (C::kCodes + C::kScales) + C::kCodes;
+                            uint32_t b[4];
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) {
+                                const int key = t + 4 * u;
+                                const int chunk = D == 128 ? (g >> 1) ^ (key & 2) : g >> 2;
+                                ld_shared<D / 64>(vc[u], from + key * (D / 2) + chunk * 16 + (g * (D / 16)) % 16);
+                                b[u] = ld_shared_u8(from + C::kCodes + C::kScales + key * (D / 16) + (D == 128 ? g : g / 2));
+                            }
+                            if (!filled(first + 16 * z))           // values that no row sees may be NaN: zeros
+#pragma unroll
+                                for (int u = 0; u < 4; ++u)
+                                    if (!wanted(first + 16 * z + t + 4 * u)) b[u] = 0;
+                            vsc[0] = scales_to_half(b[0] | (b[1] << 8));
+                            vsc[1] = scales_to_half(b[2] | (b[3] << 8));
+                        }
                         if ((m & 3) == 0) {
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
-                                const uint32_t w0 = now.v[2 * h][m / 4], w1 = now.v[2 * h + 1][m / 4];
+                                const uint32_t w0 = vc[2 * h][m / 4], w1 = vc[2 * h + 1][m / 4];
                                 codes_to_half((w0 & 0x0f0f0f0fu) | ((w1 << 4) & 0xf0f0f0f0u), vd[2 * h]);
                                 codes_to_half(((w0 >> 4) & 0x0f0f0f0fu) | (w1 & 0xf0f0f0f0u), vd[2 * h + 1]);
                             }
@@ -408,9 +522,11 @@ __global__ void __launch_bounds__(kSplitWarps * 32) attn_split_kernel(const __gr
                         a[3] = mul_half2(vd[3][m & 3], vsc[1]);
                     });
             }
-            now = ahead;
         }
+        __syncwarp();
+        stage = stage + 1 == C::kStages ? 0 : stage + 1;
     }
+    cp_async_wait<0>();
 
     // Join the four warps' results through shared memory.
     __syncthreads();
@@ -458,7 +574,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32) attn_split_kernel(const __gr
             v[1] = fmaf(f, x.y, v[1]);
         }
         if ((isnan(v[0]) || isnan(v[1])) && !isnan(total) && it.tokens > 1)
-            visible_keys_only<T, D, Q4, 2>(p, it, kt, kSplitKeys, row, base, d, v);
+            visible_keys_only<T, D, Q4, 2>(p, it, kt, C::kKeys, row, base, d, v);
         const int token = it.q0 + row / p.group, head = it.head * p.group + row % p.group;
         if (p.splits == 1) {
             const float inv = total > 0.f ? p.out_scale / total : (total == 0.f ? 0.f : total);
@@ -472,38 +588,74 @@ __global__ void __launch_bounds__(kSplitWarps * 32) attn_split_kernel(const __gr
     }
 }
 
-// Joins the splits' partial results: one warp per row.
+// Joins the splits' partial results: a CTA per row, its warps take every fourth split. The weights of
+// the splits come first, so that the loads of the partial rows do not wait for each other.
+constexpr int kJoinWarps = 4;
+
 template <typename T, int D>
-__global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const __grid_constant__ AttnParams p) {
+    __shared__ float weight[kMaxSplits];
+    __shared__ float part[kJoinWarps][D];
+    griddep_launch_dependents();
     griddep_wait();
-    const int lane = threadIdx.x & 31;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    if (row >= static_cast<int64_t>(p.num_tokens) * p.heads) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t row = blockIdx.x;
     const int token = static_cast<int>(row / p.heads), head = static_cast<int>(row - static_cast<int64_t>(token) * p.heads);
     if (p.cu != nullptr && (token < p.cu[0] || token >= p.cu[p.num_seqs])) return;     // no sequence's row
     const float2* ml = reinterpret_cast<const float2*>(p.ws_ml) + row * p.splits;
-    float top = -INFINITY;
-    for (int i = lane; i < p.splits; i += 32) top = fmaxf(top, ml[i].x);
+    // Every warp finds the maximum and the sum itself; warp 0 leaves the weights for all.
+    constexpr int kPer = kMaxSplits / 32;
+    float2 x[kPer];
+    float top = -INFINITY, total = 0.f;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        x[k] = lane + 32 * k < p.splits ? ml[lane + 32 * k] : make_float2(-INFINITY, 0.f);
+        top = fmaxf(top, x[k].x);
+    }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
     const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        // A split that saw no key of the row counts nothing, whatever its values.
+        const float f = x[k].y == 0.f ? 0.f : exp2_approx(x[k].x - base);
+        total = fmaf(f, x[k].y, total);
+        if (warp == 0) weight[lane + 32 * k] = f;
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(~0u, total, d);
+    __syncthreads();
     constexpr int N = D / 32;
-    float acc[N], total = 0.f;
+    float acc[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) acc[k] = 0.f;
-    for (int i = 0; i < p.splits; ++i) {
-        const float2 x = ml[i];
-        const float f = exp2_approx(x.x - base);
-        total = fmaf(f, x.y, total);
-        if (x.y == 0.f) continue;                       // this split saw no key of the row
-        const float* o = p.ws_o + (row * p.splits + i) * D + lane * N;
+    const float* o = p.ws_o + row * p.splits * D + lane * N;
+#pragma unroll 8
+    for (int i = warp; i < p.splits; i += kJoinWarps) {
+        float v[N];
+        if constexpr (N == 4) {
+            const float4 w = __ldcg(reinterpret_cast<const float4*>(o + static_cast<int64_t>(i) * D));
+            v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
+        } else {
+            const float2 w = __ldcg(reinterpret_cast<const float2*>(o + static_cast<int64_t>(i) * D));
+            v[0] = w.x, v[1] = w.y;
+        }
+        const float f = weight[i];
 #pragma unroll
-        for (int k = 0; k < N; ++k) acc[k] = fmaf(f, o[k], acc[k]);
+        for (int k = 0; k < N; ++k)
+            if (f != 0.f) acc[k] = fmaf(f, v[k], acc[k]);
     }
-    const float inv = total == 0.f ? 0.f : p.out_scale / total;
-    uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + token * p.o_token_stride + head * p.o_head_stride) + lane * (N / 2);
 #pragma unroll
-    for (int k = 0; k < N; k += 2) dst[k / 2] = total == 0.f ? 0u : Pair<T>::pack(acc[k] * inv, acc[k + 1] * inv);
+    for (int k = 0; k < N; ++k) part[warp][lane * N + k] = acc[k];
+    __syncthreads();
+    if (threadIdx.x < D / 2) {
+        const float inv = total == 0.f ? 0.f : p.out_scale / total;
+        float a = 0.f, b = 0.f;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) a += part[w][2 * threadIdx.x], b += part[w][2 * threadIdx.x + 1];
+        reinterpret_cast<uint32_t*>(p.out + token * p.o_token_stride + head * p.o_head_stride)[threadIdx.x] =
+            total == 0.f ? 0u : Pair<T>::pack(a * inv, b * inv);
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -528,7 +680,7 @@ template <typename T, int D>
 static int join(const AttnParams& p, cudaStream_t stream) {
     const int64_t rows = static_cast<int64_t>(p.num_tokens) * p.heads;
     cudaLaunchAttribute attr;
-    cudaLaunchConfig_t cfg = launch_config(dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, stream, &attr);
+    cudaLaunchConfig_t cfg = launch_config(dim3(static_cast<unsigned>(rows)), kJoinWarps * 32, 0, stream, &attr);
     KVX_CUDA(cudaLaunchKernelEx(&cfg, attn_join_kernel<T, D>, p), "launch attention join kernel");
     return KVX_OK;
 }
@@ -540,7 +692,7 @@ int launch_attn_join(const AttnParams& p, int head_dim, int dtype, cudaStream_t 
 
 template <typename T, int D, int NT, bool Q4>
 static int run_split(const AttnParams& p, int device, cudaStream_t stream) {
-    constexpr int smem = SplitConfig<D, Q4>::smem(8 * NT);
+    constexpr int smem = SplitConfig<D, NT, Q4>::kSmem;
     if constexpr (smem > 48 * 1024) {
         static std::atomic<uint64_t> done{0};               // devices that have the opt-in
         const uint64_t bit = 1ull << device;

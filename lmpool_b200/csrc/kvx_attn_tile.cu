@@ -36,7 +36,7 @@
 // two), so that the products see one type.
 //
 // Exponentials: the special-function unit gives 16 a clock and SM, which alone is as
-// long as the products of a tile. So 3 of 8 are computed as 2^n p(f), x = n + f, |f| <=
+// long as the products of a tile. So some are computed as 2^n p(f), x = n + f, |f| <=
 // 1/2, on the FMA units, with a degree-4 polynomial (relative error 2.8e-6, from a
 // weighted least-squares fit of 2^f; the weights are rounded to 2^-8 or 2^-11).
 //
@@ -60,7 +60,10 @@ constexpr int kTileThreads = 640;
 constexpr int kTileKeys = 128;
 constexpr int kStepKeys = 64;                  // keys of a step
 constexpr int kHalfRows = 128;                 // rows of one of the two row tiles
-constexpr int kFmaPairs = 3;                   // of 8 pairs of exponentials, on the FMA units
+// Of 8 pairs of exponentials, on the FMA units: 3 on a 16-bit cache (8 prompts of 2048: 315 us, 338 with none), 1
+// on a 4-bit one, where the widening wants the issue slots (prompts on a 4-bit cache: 401 us, 422 with 3).
+template <bool Q4>
+constexpr int kFmaPairs = Q4 ? 1 : 3;
 constexpr uint32_t kMaxWaitPolls = 1u << 22;   // each poll may suspend for a hardware-chosen time
 
 template <int D, bool Q4>
@@ -947,7 +950,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                         const uint64_t e = fma2(pair2(__uint_as_float(sr[c + 2 * k]), __uint_as_float(sr[c + 2 * k + 1])),
                                                 scale2, ref2);
                         uint64_t y;
-                        if ((k & 7) < kFmaPairs) {
+                        if ((k & 7) < kFmaPairs<Q4>) {
                             y = exp2_fma(e);
                         } else {
                             const float2 v = unpair(e);
