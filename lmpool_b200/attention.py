@@ -272,41 +272,45 @@ def load_kvcache_q4(
 # ---------------------------------------------------------------------------
 
 @functools.lru_cache(maxsize=1024)
-def _attention_workspace(device: int, args: bytes) -> int:
+def _attention_workspace(device: int, ragged: bool, sizes: tuple) -> int:
+    """Bytes of scratch that a call needs: its sizes alone decide."""
     out = ctypes.c_uint64(0)
+    args = _capi.pack_attention(0, 0, 0, 0, 0, 0, int(ragged), *(0,) * 8, 1, *sizes)
     _capi.check(_capi.lib().kvx_attention_workspace(device, args, ctypes.byref(out)), "kvx_attention_workspace")
     return out.value
 
 
 def _paged_attention(query, k_cache, v_cache, block_tables, context_lens, block_size, cu_seqlens_q, scale, window, sinks,
                      out, bits, k_scale, v_scale):
+    # This runs once a layer and step: what follows is written for few interpreter steps.
     if query.dim() != 3:
         raise RuntimeError("query must be [num_tokens, num_heads, head_dim]")
     T, heads, D = query.shape
     dtype = query.dtype
-    if dtype not in _DTYPE_CODE:
+    code = _DTYPE_CODE.get(dtype)
+    if code is None:
         raise TypeError(f"query must be bfloat16 or float16, got {dtype}")
     if D != 64 and D != 128:
         raise RuntimeError(f"head_dim must be 64 or 128, got {D}")
+    st = k_cache.stride()
     if bits == 4:
         _q4_check(k_cache, v_cache, block_size, D)
-        st = k_cache.stride()
         block_stride, slot_stride, head_stride = st[0], 0, 0
     else:
         if k_cache.dtype != dtype or v_cache.dtype != dtype:
             raise TypeError("query and cache dtypes must match")
-        if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+        shape = k_cache.shape
+        if len(shape) != 4 or shape != v_cache.shape:
             raise RuntimeError("k_cache and v_cache must both be [num_blocks, block_size, num_kv_heads, head_dim]")
-        st = k_cache.stride()
         if st != v_cache.stride():
             raise RuntimeError("k_cache and v_cache must have the same strides")
-        if k_cache.shape[1] != block_size or k_cache.shape[3] != D:
+        if shape[1] != block_size or shape[3] != D:
             raise RuntimeError(f"the cache's pages [block_size, num_kv_heads, head_dim] do not match block_size "
                                f"{block_size} and head_dim {D}")
         if st[3] != 1:
             raise RuntimeError("the cache's head_dim must be contiguous")
         block_stride, slot_stride, head_stride = 2 * st[0], 2 * st[1], 2 * st[2]
-    kv_heads = k_cache.shape[2]
+    num_blocks, _, kv_heads, _ = k_cache.shape
     if kv_heads == 0 or heads % kv_heads:
         raise RuntimeError(f"{heads} query heads are no multiple of {kv_heads} kv heads")
     if block_tables.dtype != torch.int32 or context_lens.dtype != torch.int32:
@@ -314,15 +318,20 @@ def _paged_attention(query, k_cache, v_cache, block_tables, context_lens, block_
     if block_tables.dim() != 2 or context_lens.dim() != 1 or block_tables.shape[0] != context_lens.shape[0]:
         raise RuntimeError("block_tables must be [num_seqs, width] and context_lens [num_seqs]")
     S, width = block_tables.shape
-    if width > 1 and block_tables.stride(1) != 1:
+    table_stride, step = block_tables.stride()
+    if width > 1 and step != 1:
         block_tables = block_tables.contiguous()
+        table_stride = width
     if S > 1 and context_lens.stride(0) != 1:
         context_lens = context_lens.contiguous()
+    device = query.get_device()
+    if device < 0 or device != k_cache.get_device() or device != v_cache.get_device() \
+            or device != block_tables.get_device() or device != context_lens.get_device():
+        _device_of(query, k_cache, v_cache, block_tables, context_lens)      # says which
     cu = 0
     if cu_seqlens_q is None:
         if T != S:
             raise RuntimeError(f"without cu_seqlens_q every sequence has one token: {T} tokens, {S} sequences")
-        device = _device_of(query, k_cache, v_cache, block_tables, context_lens)
     else:
         if cu_seqlens_q.dtype != torch.int32:
             raise TypeError(f"cu_seqlens_q must be int32, got {cu_seqlens_q.dtype}")
@@ -330,21 +339,21 @@ def _paged_attention(query, k_cache, v_cache, block_tables, context_lens, block_
             raise RuntimeError(f"cu_seqlens_q must hold num_seqs + 1 = {S + 1} entries")
         if S > 0 and cu_seqlens_q.stride(0) != 1:
             cu_seqlens_q = cu_seqlens_q.contiguous()
-        device = _device_of(query, k_cache, v_cache, block_tables, context_lens, cu_seqlens_q)
+        _device_of(query, cu_seqlens_q)
         cu = cu_seqlens_q.data_ptr()
-    if window is not None and window <= 0:
+    if window is None:
+        window = 0
+    elif window <= 0:
         raise ValueError(f"window must be positive (None: every key), got {window}")
     if sinks < 0:
         raise ValueError(f"sinks must not be negative, got {sinks}")
-    # Positions are 32-bit: a window or sinks beyond them are all the same.
-    window = 0 if window is None else min(int(window), 2 ** 31 - 1)
-    sinks = min(int(sinks), 2 ** 31 - 1)
     qs = query.stride()
     if qs[2] != 1 or qs[0] % 8 or qs[1] % 8 or query.data_ptr() % 16:
         query = query.contiguous() if not query.is_contiguous() else query.clone()
         qs = query.stride()
     if out is None:
         out = torch.empty((T, heads, D), dtype=dtype, device=query.device)
+        os = (heads * D, D)
     else:
         if out.shape != query.shape or out.dtype != dtype:
             raise RuntimeError("out must have query's shape and dtype")
@@ -352,26 +361,28 @@ def _paged_attention(query, k_cache, v_cache, block_tables, context_lens, block_
         os = out.stride()
         if os[2] != 1 or os[0] % 8 or os[1] % 8 or out.data_ptr() % 16:
             raise RuntimeError("out must have contiguous, 16-byte aligned rows of head_dim")
-    os = out.stride()
     if T == 0 or S == 0:
         return out
-    sizes = (T, S, heads, kv_heads, D, block_size, width, _DTYPE_CODE[dtype], bits, window, sinks,
-             D ** -0.5 if scale is None else float(scale), k_scale, v_scale, 0, 0)
-    pointers = (query.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(),
-                context_lens.data_ptr(), cu, 2 * qs[0], 2 * qs[1], 2 * os[0], 2 * os[1], block_stride, slot_stride,
-                head_stride, block_tables.stride(0), k_cache.shape[0])
-    # Sizes alone decide how much workspace a call needs.
-    need = _attention_workspace(device, _capi.pack_attention(*_NO_POINTERS[cu != 0], *sizes))
-    workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
+    # Positions are 32-bit: a window or sinks beyond them are all the same.
+    sizes = (T, S, heads, kv_heads, D, block_size, width, code, bits, min(window, _INT_MAX), min(sinks, _INT_MAX),
+             D ** -0.5 if scale is None else scale, k_scale, v_scale, 0, 0)
+    need = _attention_workspace(device, cu != 0, sizes)
+    workspace = None
+    if need:
+        scratch = torch.empty(need, dtype=torch.uint8, device=query.device)
+        workspace = scratch.data_ptr()
     rc = _capi.lib().kvx_paged_attention(
-        device, _capi.pack_attention(*pointers, *sizes), workspace.data_ptr() if need else None, need,
-        _status_word(device).data_ptr(), _raw_stream(device))
+        device,
+        _capi.pack_attention(query.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                             block_tables.data_ptr(), context_lens.data_ptr(), cu, 2 * qs[0], 2 * qs[1], 2 * os[0],
+                             2 * os[1], block_stride, slot_stride, head_stride, table_stride, num_blocks, *sizes),
+        workspace, need, _status_word(device).data_ptr(), _raw_stream(device))
     if rc:
         _capi.check(rc, "kvx_paged_attention")
     return out
 
 
-_NO_POINTERS = {False: (0,) * 15 + (1,), True: (0,) * 6 + (1,) + (0,) * 8 + (1,)}
+_INT_MAX = 2 ** 31 - 1
 
 
 def paged_attention(

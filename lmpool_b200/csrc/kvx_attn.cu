@@ -13,7 +13,7 @@ namespace kvx {
 
 constexpr int kWaves = 4;
 constexpr int kMinKeys = 512;
-constexpr int kFewRows = 32;            // rows of an item of the split kernel, at most
+constexpr int kFewRows = 32;            // rows of a sequence and kv head up to which the split kernel is taken
 constexpr int kTileRows = 256;          // rows of an item of the tile kernel
 
 struct AttnPlan {
@@ -71,19 +71,31 @@ static AttnPlan plan_of(const kvx_attention* a, int sms) {
     const int group = a->num_heads / a->num_kv_heads;
     const int64_t tokens = a->num_tokens, seqs = std::max(1, a->num_seqs);
     const int64_t avg = (tokens + seqs - 1) / seqs;
-    pl.tile = avg * group > kFewRows;
+    pl.tile = avg * group > kFewRows || group > 32;
     int keys_per_tile, fill, min_tiles;
     if (pl.tile) {
-        pl.tile_tokens = kTileRows / group;
+        // Sequences of few rows: items of one row tile, the other half of the kernel rests.
+        pl.tile_tokens = (avg * group <= kTileRows / 2 ? kTileRows / 2 : kTileRows) / group;
         keys_per_tile = 128;
         fill = sms;
         min_tiles = 4;
     } else {
-        pl.nt = avg * group <= 8 ? 1 : avg * group <= 16 ? 2 : 4;
-        pl.tile_tokens = a->cu_seqlens_q ? std::max(1, 8 * pl.nt / group) : 1;
+        // The row tiles of an item: the choice that reads the keys for the least work, a pass over them costing
+        // about as much as three row tiles (the widening and the loads).
+        int64_t least = INT64_MAX;
+        for (int nt = 1; nt <= 4; ++nt) {
+            if (8 * nt < group) continue;
+            const int per = a->cu_seqlens_q ? 8 * nt / group : 1;
+            const int64_t cost = (avg + per - 1) / per * (3 + nt);
+            if (cost < least) {
+                least = cost;
+                pl.nt = nt;
+                pl.tile_tokens = per;
+            }
+        }
         const bool q4 = a->cache_bits == 4;
-        keys_per_tile = q4 && pl.nt < 4 ? 128 : 64;
-        fill = sms * (q4 ? (pl.nt == 1 ? 4 : pl.nt == 2 ? 3 : 2) : 2) * kWaves;
+        keys_per_tile = q4 && pl.nt < 3 ? 128 : 64;
+        fill = sms * (q4 && pl.nt == 1 ? 4 : 2) * kWaves;
         min_tiles = kMinKeys / keys_per_tile;
     }
     pl.tile_slots = static_cast<int>(a->cu_seqlens_q ? tokens / pl.tile_tokens + a->num_seqs : a->num_seqs);

@@ -301,7 +301,7 @@ __device__ __noinline__ void visible_scores(const AttnParams& p, const AttnItem&
 // Launches (one translation unit per kernel family)
 // ---------------------------------------------------------------------------
 
-// Rows are few: keys split over CTAs and warps (kvx_attn_split.cu). An item has 8 * nt rows (nt = 1, 2, 4).
+// Rows are few: keys split over CTAs and warps (kvx_attn_split.cu). An item has 8 * nt rows (nt = 1 to 4).
 int launch_attn_split(const AttnParams& p, int head_dim, int dtype, bool q4, int nt, int device, cudaStream_t stream);
 // Rows are many: 256-row tiles on the tensor cores (kvx_attn_tile.cu).
 int launch_attn_tile(const AttnParams& p, int head_dim, int dtype, bool q4, int device, int sms, cudaStream_t stream);

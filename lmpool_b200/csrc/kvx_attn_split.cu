@@ -101,7 +101,7 @@ __device__ __forceinline__ uint32_t ld_shared_u8(uint32_t addr) {
 
 template <int D, int NT, bool Q4>
 struct SplitConfig {
-    static constexpr int kSlices = Q4 && NT < 4 ? kQ4Slices : 1;             // slices of 16 keys a warp takes at once
+    static constexpr int kSlices = Q4 && NT < 3 ? kQ4Slices : 1;             // slices of 16 keys a warp takes at once
     static constexpr int kWarpKeys = 16 * kSlices;
     static constexpr int kKeys = kWarpKeys * kSplitWarps;                    // keys of a tile
     static constexpr int kStages = Q4 ? kQ4Stages : 3;
@@ -714,6 +714,7 @@ static int run_rows(const AttnParams& p, int nt, int device, cudaStream_t stream
     switch (nt) {
         case 1: return run_split<T, D, 1, Q4>(p, device, stream);
         case 2: return run_split<T, D, 2, Q4>(p, device, stream);
+        case 3: return run_split<T, D, 3, Q4>(p, device, stream);
         default: return run_split<T, D, 4, Q4>(p, device, stream);
     }
 }

@@ -311,7 +311,7 @@ struct TileBars {
     uint64_t q_full, q_empty;
     uint64_t s_full[2][2], p_full[2][2];     // [row tile][score buffer]
     uint64_t pv_done[2], o_full[2], o_free[2], sums_full[2];
-    uint64_t drain;
+    uint64_t drain, idle;
     uint64_t work_full[kWork], work_empty[kWork];
     TileWork work[kWork];
     uint32_t raw_bad[4];       // 16-key groups of a raw tile that were not copied
@@ -345,15 +345,70 @@ struct Ring {
     }
 };
 
-__device__ __forceinline__ AttnItem tile_item(const AttnParams& p, int x) {
-    const int per_slot = p.kv_heads * p.splits;
-    const int slot = x / per_slot, rest = x - slot * per_slot;
-    // The last tokens of a prompt see the most keys: their items go first.
-    AttnItem it = locate_item(p, p.tile_slots - 1 - slot);
-    it.head = rest / p.splits;
-    it.split = rest - it.head * p.splits;
-    return it;
-}
+// The items of a call, without gaps, as one warp walks them: tiles of queries from the last sequence's
+// last to the first (the last tokens of a prompt see the most keys: they go first), and of
+// each every kv head and split. Sequences are counted 32 at a time, one a lane; the walk only
+// goes on, so that it passes over them once.
+struct ItemWalk {
+    int chunk;      // sequences 32 * chunk ... are in view
+    int after;      // tiles of the sequences behind them
+    int tiles;      // this lane's sequence: its tiles
+    int upto;       // and those of the lanes from here on
+    int all;        // tiles of the 32
+
+    __device__ __forceinline__ int tiles_of(const AttnParams& p, int s, bool report) const {
+        if (s >= p.num_seqs) return 0;
+        if (p.cu == nullptr) return 1;
+        const int a = p.cu[s], b = p.cu[s + 1];
+        if (a < 0 || b < a || b > p.num_tokens) {
+            if (report) atomicOr(p.status, KVX_DEV_BAD_LEN);
+            return 0;
+        }
+        return (b - a + p.tile_tokens - 1) / p.tile_tokens;
+    }
+    __device__ __forceinline__ void view(const AttnParams& p, int c) {
+        const int lane = threadIdx.x & 31;
+        chunk = c;
+        tiles = tiles_of(p, 32 * c + lane, false);
+        upto = tiles;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int other = __shfl_down_sync(~0u, upto, d);
+            if (lane + d < 32) upto += other;
+        }
+        all = __shfl_sync(~0u, upto, 0);
+    }
+    // Starts the walk; the number of tiles of the call.
+    __device__ __forceinline__ int64_t start(const AttnParams& p) {
+        int64_t n = 0;
+        for (int s = threadIdx.x & 31; s < p.num_seqs; s += 32) n += tiles_of(p, s, true);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) n += __shfl_xor_sync(~0u, n, d);
+        after = 0;
+        view(p, (p.num_seqs - 1) / 32);
+        return n;
+    }
+    // Tile y (counted from the end), not before an earlier call's.
+    __device__ __forceinline__ AttnItem tile(const AttnParams& p, int y) {
+        while (y >= after + all && chunk > 0) {
+            after += all;
+            view(p, chunk - 1);
+        }
+        const int rest = y - after;                                  // in this chunk, from its end
+        const uint32_t hit = __ballot_sync(~0u, rest < upto && rest >= upto - tiles);
+        const int who = hit ? __ffs(hit) - 1 : 0;
+        const int tile = __shfl_sync(~0u, upto - 1 - rest, who);     // of its sequence, from its start
+        AttnItem it;
+        it.seq = 32 * chunk + who;
+        it.head = it.split = 0;
+        const int a = p.cu ? p.cu[it.seq] : it.seq, len = p.cu ? p.cu[it.seq + 1] - a : 1;
+        const int first = tile * p.tile_tokens;
+        it.q0 = a + first;
+        it.tokens = hit ? min(p.tile_tokens, len - first) : 0;
+        it.pos0 = context_of(p, it.seq) - len + first;
+        return it;
+    }
+};
 
 // Writes a row again from its visible keys alone (see visible_keys_only).
 template <typename T, int D, bool Q4>
@@ -375,6 +430,9 @@ __device__ __noinline__ void visible_row(const AttnParams& p, const AttnItem& it
     }
 }
 
+// Whether an item has rows in its second row tile.
+__device__ __forceinline__ bool second_tile(const AttnParams& p, const AttnItem& it) { return it.tokens * p.group > kHalfRows; }
+
 // Whether a tile of a 16-bit cache is gathered row by row: always without TMA, else the value
 // tile (odd op) that reaches behind the context.
 __device__ __forceinline__ bool gathered(int box_rows, int op, int first, int last) {
@@ -385,8 +443,7 @@ __device__ __forceinline__ bool gathered(int box_rows, int op, int first, int la
 // ring, raw pages of a 4-bit cache into the ring of raw tiles. A lane looks up one box or run
 // of 16 keys and copies it, so that a tile's page lookups are in flight together.
 template <int D, bool Q4>
-__device__ __forceinline__ void issue_copies(const AttnParams& p, const TileMaps& maps, uint32_t base, TileBars<D, Q4>* bars,
-                                             int items) {
+__device__ __forceinline__ void issue_copies(const AttnParams& p, const TileMaps& maps, uint32_t base, TileBars<D, Q4>* bars) {
     using C = TileConfig<D, Q4>;
     Ring<Q4 ? C::kRawStages : C::kStages> ring;
     uint32_t* abort = &bars->abort;
@@ -394,7 +451,7 @@ __device__ __forceinline__ void issue_copies(const AttnParams& p, const TileMaps
     const int run = Q4 ? 16 : maps.box_rows;            // keys of a copy
     const int at = lane * run;                          // this lane's first key in a tile
     Ring<kWork> work;
-    for (int x = blockIdx.x; x < items; x += gridDim.x) {
+    while (true) {
         AttnItem it;
         KeyTiles kt;
         if (!take_work(bars, work, p.status, it, kt)) return;
@@ -453,7 +510,8 @@ __device__ __forceinline__ void issue_copies(const AttnParams& p, const TileMaps
     }
 }
 
-// The next item of a role (a whole warp), copied out of the ring that warp 14 fills.
+// The next item of a role (a whole warp), copied out of the ring that warp 14 fills; false after the last
+// one, or when the CTA gave up.
 template <int D, bool Q4>
 __device__ __forceinline__ bool take_work(TileBars<D, Q4>* bars, Ring<kWork>& ring, int32_t* status, AttnItem& it, KeyTiles& kt) {
     if (!warp_wait(&bars->work_full[ring.at], ring.phase, &bars->abort, status)) return false;
@@ -462,7 +520,7 @@ __device__ __forceinline__ bool take_work(TileBars<D, Q4>* bars, Ring<kWork>& ri
     __syncwarp();
     if ((threadIdx.x & 31) == 0) mbar_arrive(&bars->work_empty[ring.at]);
     ring.next();
-    return true;
+    return it.seq >= 0;
 }
 
 template <typename T, int D, bool Q4>
@@ -502,6 +560,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                 mbar_init(&bars->sums_full[i], 128);
             }
             mbar_init(&bars->drain, 2);
+            mbar_init(&bars->idle, 128);
             for (int i = 0; i < kWork; ++i) {
                 mbar_init(&bars->work_full[i], 1);
                 mbar_init(&bars->work_empty[i], kRoles);
@@ -516,16 +575,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
     griddep_wait();
     constexpr uint32_t tmem = 0;               // all 512 columns are this CTA's: they start at 0
     uint32_t* abort = &bars->abort;
-    const int items = p.tile_slots * p.kv_heads * p.splits;
 
     // Registers: 5 x 96 a thread at launch; from here on 2 x 128, 72, 56, and 96 for the warps that call functions.
     if (warp >= 16) {
         // ---- finished rows ----
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        uint32_t phase = 0;
+        uint32_t phases[2] = {0, 0};
         bool ok = true;
         Ring<kWork> work;
-        for (int x = blockIdx.x; x < items && ok; x += gridDim.x) {
+        while (ok) {
             AttnItem it;
             KeyTiles kt;
             if (!take_work(bars, work, p.status, it, kt)) break;
@@ -533,6 +591,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
             const int n = kt.end - kt.begin;
 #pragma unroll 1
             for (int i = 0; i < 2; ++i) {
+                if (i == 1 && !second_tile(p, it)) break;
+                const uint32_t phase = i ? phases[1] : phases[0];
                 const int row = (threadIdx.x & 127) + i * kHalfRows;
                 const int token = row / p.group, head = row - token * p.group;
                 const bool live = token < it.tokens;
@@ -583,7 +643,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                 }
                 if (live && nan && !isnan(sum)) visible_row<T, D, Q4>(p, it, kt, kTileKeys, row, dst, at);
             }
-            if (n > 0) phase ^= 1;
+            if (n > 0) {
+                phases[0] ^= 1;
+                if (second_tile(p, it)) phases[1] ^= 1;
+            }
         }
     } else if (warp >= 12) {
         give_registers<56>();
@@ -599,6 +662,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
             Ring<C::kStages> ring;
             Ring<kWork> work;
             uint32_t q_phase = 0, p_phase = 0, free_phase = 1;
+            [[maybe_unused]] uint32_t idle_phase = 0;
             // Scores against the keys of half h of a stage, into buffer h.
             auto scores = [&](int h, int stage) {
                 if (leader) {
@@ -616,7 +680,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                 if (leader) tc_commit(bar);
                 __syncwarp();
             };
-            for (int x = blockIdx.x; x < items; x += gridDim.x) {
+            while (true) {
                 AttnItem it;
                 KeyTiles kt;
                 if (!take_work(bars, work, p.status, it, kt)) break;
@@ -624,6 +688,19 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                 if (n <= 0) continue;
                 if (!warp_wait(&bars->q_full, q_phase, abort, p.status)) break;
                 q_phase ^= 1;
+                if (i == 1 && !second_tile(p, it)) {
+                    // No rows here: the stages are let go as they come.
+                    bool ok = true;
+                    for (int op = 0; op < 2 * n; ++op, ring.next()) {
+                        if (!(ok = warp_wait(&bars->full[ring.at], ring.phase, abort, p.status))) break;
+                        if (lane == 0) mbar_arrive(&bars->empty[ring.at]);
+                    }
+                    if (ok && Q4) ok = warp_wait(&bars->idle, idle_phase, abort, p.status);
+                    if (!ok) break;
+                    idle_phase ^= 1;
+                    if (lane == 0) mbar_arrive(&bars->q_empty);
+                    continue;
+                }
                 if (!warp_wait(&bars->full[ring.at], ring.phase, abort, p.status)) break;
                 tc_fence_after();
                 scores(0, ring.at);
@@ -678,18 +755,28 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
             bar_wait(&bars->drain, 0, &never, p.status);
         }
         __syncwarp();
-        if (warp == 13) issue_copies<D, Q4>(p, maps, base, bars, items);
+        if (warp == 13) issue_copies<D, Q4>(p, maps, base, bars);
         if (warp == 14) {
             Ring<kWork> ring;
-            for (int x = blockIdx.x; x < items; x += gridDim.x, ring.next()) {
-                const AttnItem it = tile_item(p, x);
-                const KeyTiles kt = key_tiles<kTileKeys>(p, it);
+            ItemWalk walk;
+            const int per_tile = p.kv_heads * p.splits;
+            const int64_t items = walk.start(p) * per_tile;
+            for (int64_t x = blockIdx.x;; x += gridDim.x, ring.next()) {
+                TileWork next = {};
+                next.it.seq = -1;                                    // no more items
+                if (x < items) {
+                    const int y = static_cast<int>(x / per_tile), rest = static_cast<int>(x - static_cast<int64_t>(y) * per_tile);
+                    next.it = walk.tile(p, y);
+                    next.it.head = rest / p.splits;
+                    next.it.split = rest - next.it.head * p.splits;
+                    next.kt = key_tiles<kTileKeys>(p, next.it);
+                }
                 if (!warp_wait(&bars->work_empty[ring.at], ring.phase ^ 1, abort, p.status)) break;
                 if (lane == 0) {
-                    bars->work[ring.at].it = it;
-                    bars->work[ring.at].kt = kt;
+                    bars->work[ring.at] = next;
                     mbar_arrive(&bars->work_full[ring.at]);
                 }
+                if (next.it.seq < 0) break;
             }
         }
     } else if (warp >= 8) {
@@ -714,7 +801,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
         }
         bool ok = true;
         Ring<kWork> work;
-        for (int x = blockIdx.x; x < items && ok; x += gridDim.x) {
+        while (ok) {
             AttnItem it;
             KeyTiles kt;
             if (!take_work(bars, work, p.status, it, kt)) break;
@@ -866,25 +953,33 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
         const uint32_t s_at = tmem + lanes + i * 2 * kStepKeys, o_at = tmem + lanes + 256 + i * D;
         const int token = row / p.group;
         const int head = row - token * p.group;
-        uint32_t s_phase = 0, q_phase = 0, free_phase = 1, pv_phase = 1;
+        [[maybe_unused]] uint32_t q_phase = 0;
+        uint32_t s_phase = 0, free_phase = 1, pv_phase = 1;
         Ring<kWork> work;
-        for (int x = blockIdx.x; x < items; x += gridDim.x) {
+        while (true) {
             AttnItem it;
             KeyTiles kt;
             if (!take_work(bars, work, p.status, it, kt)) break;
             const int n = kt.end - kt.begin;
             if (n <= 0) continue;
+            const bool idle = i == 1 && !second_tile(p, it);
+            [[maybe_unused]] float factor = 1.f;
+            if constexpr (Q4) {
+                // In idle items too, and acknowledged: a barrier's phases are told apart by parity alone, so the
+                // queries of the next item must not come before these warps have seen those of this one.
+                if (!warp_wait(&bars->q_full, q_phase, abort, p.status)) break;
+                q_phase ^= 1;
+                factor = factors[row];
+                if (idle) mbar_arrive(&bars->idle);
+            }
+            if (idle) continue;
             const bool live = token < it.tokens;
             const int pos = live ? it.pos0 + token : -1;
             const int last = it.pos0 + it.tokens - 1;
             float top = -INFINITY, sum = 0.f;                       // raw score, sum of weights
             float scale = p.scale_log2;
             bool ok = true;
-            if constexpr (Q4) {
-                if (!warp_wait(&bars->q_full, q_phase, abort, p.status)) break;
-                q_phase ^= 1;
-                scale *= factors[row];
-            }
+            if constexpr (Q4) scale *= factor;
 #pragma unroll 1
             for (int u = 0; u < 2 * n; ++u) {
                 const int h = u & 1;

@@ -33,9 +33,10 @@ struct Q4Params {
     int64_t key_token_stride, value_token_stride;   // bytes
     int64_t block_stride;
     const int64_t* slots;
-    int64_t num_tokens, num_slots;
-    int64_t items;                                  // 2 * num_tokens * groups per row
-    int32_t block_size, heads, head_dim;
+    int64_t num_slots;
+    int32_t rows;                                   // 2 * tokens: K and V of a token follow each other
+    int32_t block_rows;                             // rows of a CTA
+    int32_t block_size, block_shift, heads, head_dim;   // block_shift < 0: not a power of two
     int32_t row_groups;                             // heads * head_dim / 16
     float k_mul, v_mul;                             // store: 1 / scale, load: scale
     int32_t* status;
@@ -45,20 +46,23 @@ struct Q4Place {
     int64_t codes, scale;    // byte offsets of the group in its plane
 };
 
-// Item i: plane, token and group of the row; false where there is no row.
-__device__ __forceinline__ bool q4_item(const Q4Params& p, int64_t i, int* plane, int64_t* token, int* group) {
-    if (i >= p.items) return false;
-    const int64_t row = i / p.row_groups;
-    *group = static_cast<int>(i - row * p.row_groups);
-    *plane = row >= p.num_tokens;
-    *token = row - (*plane ? p.num_tokens : 0);
-    return true;
+// This thread's plane, token and group of the row; false where there is none.
+__device__ __forceinline__ bool q4_item(const Q4Params& p, int* plane, int64_t* token, int* group) {
+    const int in_block = static_cast<int>(threadIdx.x) / p.row_groups;
+    const int row = static_cast<int>(blockIdx.x) * p.block_rows + in_block;
+    *group = static_cast<int>(threadIdx.x) - in_block * p.row_groups + static_cast<int>(blockIdx.y) * kQ4Threads;
+    *plane = row & 1;
+    *token = row >> 1;
+    return in_block < p.block_rows && row < p.rows && *group < p.row_groups;
 }
 
 __device__ __forceinline__ Q4Place q4_place(const Q4Params& p, int64_t slot, int group) {
     const int per_head = p.head_dim / 16;
     const int head = group / per_head, g = group - head * per_head;
-    const int64_t blk = slot / p.block_size;
+    int64_t blk;
+    if (p.block_shift >= 0) blk = slot >> p.block_shift;
+    else if (p.num_slots <= INT_MAX) blk = static_cast<int>(slot) / p.block_size;
+    else blk = slot / p.block_size;
     const int off = static_cast<int>(slot - blk * p.block_size);
     const int64_t run = blk * p.block_stride + static_cast<int64_t>(head) * p.block_size * (p.head_dim / 16 * 9);
     Q4Place a;
@@ -82,7 +86,7 @@ __global__ void __launch_bounds__(kQ4Threads) store_q4_kernel(const __grid_const
     griddep_wait();
     int plane, group;
     int64_t token;
-    if (!q4_item(p, static_cast<int64_t>(blockIdx.x) * kQ4Threads + threadIdx.x, &plane, &token, &group)) return;
+    if (!q4_item(p, &plane, &token, &group)) return;
     const int64_t slot = ld_cg(p.slots + token);
     const char* src = plane ? p.value + token * p.value_token_stride : p.key + token * p.key_token_stride;
     uint32_t raw[8];
@@ -136,7 +140,7 @@ __global__ void __launch_bounds__(kQ4Threads) load_q4_kernel(const __grid_consta
     griddep_wait();
     int plane, group;
     int64_t token;
-    if (!q4_item(p, static_cast<int64_t>(blockIdx.x) * kQ4Threads + threadIdx.x, &plane, &token, &group)) return;
+    if (!q4_item(p, &plane, &token, &group)) return;
     const int64_t slot = ld_cg(p.slots + token);
     uint32_t out[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (q4_slot(p, slot, group, plane)) {
@@ -201,21 +205,26 @@ static int q4_launch(bool store, int32_t device, int32_t dtype, const void* key,
     p.value_token_stride = value_token_stride;
     p.block_stride = block_stride;
     p.slots = slots;
-    p.num_tokens = num_tokens;
     p.num_slots = num_blocks * block_size;
     p.block_size = block_size;
+    p.block_shift = -1;
+    if ((block_size & (block_size - 1)) == 0)
+        for (p.block_shift = 0; (1 << p.block_shift) < block_size;) ++p.block_shift;
     p.heads = kv_heads;
     p.head_dim = head_dim;
     p.row_groups = kv_heads * (head_dim / 16);
-    p.items = 2 * num_tokens * p.row_groups;
+    if (num_tokens > INT_MAX / 4) return fail(KVX_EINVAL, "too many tokens");
+    p.rows = static_cast<int32_t>(2 * num_tokens);
+    p.block_rows = p.row_groups < kQ4Threads ? kQ4Threads / p.row_groups : 1;
     p.k_mul = store ? 1.f / k_scale : k_scale;
     p.v_mul = store ? 1.f / v_scale : v_scale;
     p.status = status;
-    const int64_t blocks = (p.items + kQ4Threads - 1) / kQ4Threads;
-    if (blocks > INT_MAX) return fail(KVX_EINVAL, "too many tokens");
+    const dim3 grid(static_cast<unsigned>((p.rows + p.block_rows - 1) / p.block_rows),
+                    static_cast<unsigned>((p.row_groups + kQ4Threads - 1) / kQ4Threads));
+    if (grid.y > 65535) return fail(KVX_EINVAL, "rows of kv_heads * head_dim are too long");
     KVX_DEVICE_GUARD(device);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(kQ4Threads);
     cfg.stream = static_cast<cudaStream_t>(stream);
     cudaLaunchAttribute attr[1];
