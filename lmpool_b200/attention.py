@@ -27,7 +27,7 @@ import functools
 import torch
 
 from . import _capi
-from .kv_transfer import _status_word
+from .kv_transfer import _STATUS, _status_word
 
 
 def _cache_strides(k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, int]:
@@ -151,6 +151,16 @@ def store_kvcache_layers(
 _DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1}
 
 
+def _status(device: int) -> int:
+    """Address of the device's status word. Its first use allocates it, which a graph's capture must not record."""
+    word = _STATUS.get(device)
+    if word is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("make the first call on a device before capturing a graph")
+        word = _status_word(device)
+    return word.data_ptr()
+
+
 def q4_row_bytes(head_dim: int) -> int:
     """Bytes of one token's row of one kv head in a 4-bit cache: ``head_dim / 2`` of codes and ``head_dim / 16``
     of scales. A 4-bit cache is a ``uint8`` tensor ``[..., N, block_size, H, q4_row_bytes(D)]``; inside a page the
@@ -227,8 +237,9 @@ def store_kvcache_q4(
     key, value = _rows_of(key), _rows_of(value)
     rc = _capi.lib().kvx_store_kvcache_q4(
         device, _DTYPE_CODE[key.dtype], key.data_ptr(), value.data_ptr(), key.stride(0) * 2, value.stride(0) * 2,
-        k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), slot_mapping.data_ptr(), T, k_cache.shape[0],
-        int(block_size), H, D, k_scale, v_scale, _status_word(device).data_ptr(), _raw_stream(device))
+        k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0) if k_cache.shape[0] > 1 else 0, slot_mapping.data_ptr(), T,
+        k_cache.shape[0],
+        int(block_size), H, D, k_scale, v_scale, _status(device), _raw_stream(device))
     if rc:
         _capi.check(rc, "kvx_store_kvcache_q4")
 
@@ -260,8 +271,9 @@ def load_kvcache_q4(
         return key, value
     rc = _capi.lib().kvx_load_kvcache_q4(
         device, _DTYPE_CODE[dtype], key.data_ptr(), value.data_ptr(), H * D * 2, H * D * 2, k_cache.data_ptr(),
-        v_cache.data_ptr(), k_cache.stride(0), slot_mapping.data_ptr(), T, k_cache.shape[0], int(block_size), H, D,
-        k_scale, v_scale, _status_word(device).data_ptr(), _raw_stream(device))
+        v_cache.data_ptr(), k_cache.stride(0) if k_cache.shape[0] > 1 else 0, slot_mapping.data_ptr(), T, k_cache.shape[0],
+        int(block_size), H, D,
+        k_scale, v_scale, _status(device), _raw_stream(device))
     if rc:
         _capi.check(rc, "kvx_load_kvcache_q4")
     return key, value
@@ -295,7 +307,7 @@ def _paged_attention(query, k_cache, v_cache, block_tables, context_lens, block_
     st = k_cache.stride()
     if bits == 4:
         _q4_check(k_cache, v_cache, block_size, D)
-        block_stride, slot_stride, head_stride = st[0], 0, 0
+        block_stride, slot_stride, head_stride = st[0] if k_cache.shape[0] > 1 else 0, 0, 0
     else:
         if k_cache.dtype != dtype or v_cache.dtype != dtype:
             raise TypeError("query and cache dtypes must match")
@@ -309,7 +321,10 @@ def _paged_attention(query, k_cache, v_cache, block_tables, context_lens, block_
                                f"{block_size} and head_dim {D}")
         if st[3] != 1:
             raise RuntimeError("the cache's head_dim must be contiguous")
-        block_stride, slot_stride, head_stride = 2 * st[0], 2 * st[1], 2 * st[2]
+        # The stride of a dimension of one entry is not used and may be anything.
+        block_stride = 2 * st[0] if shape[0] > 1 else 2 * D * block_size * shape[2]
+        slot_stride = 2 * st[1] if block_size > 1 else 2 * D * shape[2]
+        head_stride = 2 * st[2] if shape[2] > 1 else 2 * D
     num_blocks, _, kv_heads, _ = k_cache.shape
     if kv_heads == 0 or heads % kv_heads:
         raise RuntimeError(f"{heads} query heads are no multiple of {kv_heads} kv heads")
@@ -352,7 +367,7 @@ def _paged_attention(query, k_cache, v_cache, block_tables, context_lens, block_
         query = query.contiguous() if not query.is_contiguous() else query.clone()
         qs = query.stride()
     if out is None:
-        out = torch.empty((T, heads, D), dtype=dtype, device=query.device)
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
         os = (heads * D, D)
     else:
         if out.shape != query.shape or out.dtype != dtype:
@@ -361,6 +376,8 @@ def _paged_attention(query, k_cache, v_cache, block_tables, context_lens, block_
         os = out.stride()
         if os[2] != 1 or os[0] % 8 or os[1] % 8 or out.data_ptr() % 16:
             raise RuntimeError("out must have contiguous, 16-byte aligned rows of head_dim")
+        if out.data_ptr() == query.data_ptr() and T:
+            raise RuntimeError("out must not be the query")
     if T == 0 or S == 0:
         return out
     # Positions are 32-bit: a window or sinks beyond them are all the same.
@@ -376,7 +393,7 @@ def _paged_attention(query, k_cache, v_cache, block_tables, context_lens, block_
         _capi.pack_attention(query.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                              block_tables.data_ptr(), context_lens.data_ptr(), cu, 2 * qs[0], 2 * qs[1], 2 * os[0],
                              2 * os[1], block_stride, slot_stride, head_stride, table_stride, num_blocks, *sizes),
-        workspace, need, _status_word(device).data_ptr(), _raw_stream(device))
+        workspace, need, _status(device), _raw_stream(device))
     if rc:
         _capi.check(rc, "kvx_paged_attention")
     return out
@@ -411,7 +428,7 @@ def paged_attention(
     from 0) sequence ``s`` has the tokens ``cu_seqlens_q[s]`` to ``cu_seqlens_q[s + 1]``, the last of its context:
     prompts, chunks of prompts, drafted tokens. Token at position ``p`` sees key ``j <= p`` if ``window`` is None, if
     ``p - j < window`` or if ``j < sinks``. A token that sees no key gets zeros. Rows behind the last sequence are left
-    as they were. ``scale`` (default ``D ** -0.5``) must be positive.
+    as they were. ``out`` takes the result and must not overlap the inputs. ``scale`` (default ``D ** -0.5``) must be positive.
 
     Runs on the current stream without synchronising; lengths and tables are read on the device, so a captured call
     can be replayed with others. Bad page ids (their keys read as zeros) and lengths are recorded in the device's

@@ -13,7 +13,12 @@ namespace kvx {
 
 constexpr int kWaves = 4;
 constexpr int kMinKeys = 512;
-constexpr int kFewRows = 32;            // rows of a sequence and kv head up to which the split kernel is taken
+// Rows of a sequence and kv head (tokens x group heads) up to which the split kernel is taken. Split against tile
+// kernel, us, bf16, 8 kv heads of 128: 16-bit cache, 32 sequences of 2000 keys: 12 rows 83/79, 16 rows 87/79,
+// 24 rows 99/77; 256 of 600: 151/168, 157/167, 189/169; 4 of 30000: 114/120, 118/118, 130/118. 4-bit cache: 16 rows
+// 69/99, 24 rows 91/99, 32 rows 122/99; 133/167, 177/232, 241/232; 83/157, 110/157, 146/161.
+constexpr int kFewRows16 = 16;
+constexpr int kFewRows4 = 24;
 constexpr int kTileRows = 256;          // rows of an item of the tile kernel
 
 struct AttnPlan {
@@ -22,6 +27,7 @@ struct AttnPlan {
     int tile_tokens;
     int tile_slots;
     int splits;
+    int min_tiles;      // key tiles of a split, at least
     uint64_t workspace;
 };
 
@@ -71,19 +77,19 @@ static AttnPlan plan_of(const kvx_attention* a, int sms) {
     const int group = a->num_heads / a->num_kv_heads;
     const int64_t tokens = a->num_tokens, seqs = std::max(1, a->num_seqs);
     const int64_t avg = (tokens + seqs - 1) / seqs;
-    pl.tile = avg * group > kFewRows || group > 32;
-    int keys_per_tile, fill, min_tiles;
+    pl.tile = avg * group > (a->cache_bits == 4 ? kFewRows4 : kFewRows16);
+    int keys_per_tile, fill;
     if (pl.tile) {
         // Sequences of few rows: items of one row tile, the other half of the kernel rests.
         pl.tile_tokens = (avg * group <= kTileRows / 2 ? kTileRows / 2 : kTileRows) / group;
         keys_per_tile = 128;
         fill = sms;
-        min_tiles = 4;
+        pl.min_tiles = 4;
     } else {
         // The row tiles of an item: the choice that reads the keys for the least work, a pass over them costing
         // about as much as three row tiles (the widening and the loads).
         int64_t least = INT64_MAX;
-        for (int nt = 1; nt <= 4; ++nt) {
+        for (int nt = 1; nt <= 3; ++nt) {
             if (8 * nt < group) continue;
             const int per = a->cu_seqlens_q ? 8 * nt / group : 1;
             const int64_t cost = (avg + per - 1) / per * (3 + nt);
@@ -96,7 +102,7 @@ static AttnPlan plan_of(const kvx_attention* a, int sms) {
         const bool q4 = a->cache_bits == 4;
         keys_per_tile = q4 && pl.nt < 3 ? 128 : 64;
         fill = sms * (q4 && pl.nt == 1 ? 4 : 2) * kWaves;
-        min_tiles = kMinKeys / keys_per_tile;
+        pl.min_tiles = kMinKeys / keys_per_tile;
     }
     pl.tile_slots = static_cast<int>(a->cu_seqlens_q ? tokens / pl.tile_tokens + a->num_seqs : a->num_seqs);
     const int64_t items = std::max<int64_t>(seqs, (tokens + pl.tile_tokens - 1) / pl.tile_tokens) * a->num_kv_heads;
@@ -106,7 +112,7 @@ static AttnPlan plan_of(const kvx_attention* a, int sms) {
         keys = std::min(keys, static_cast<int64_t>(a->window) + a->sinks + pl.tile_tokens + 2 * keys_per_tile);
     const int64_t tiles = (keys + keys_per_tile - 1) / keys_per_tile;
     int64_t splits = fill / std::max<int64_t>(1, items);
-    splits = std::min(splits, tiles / min_tiles);
+    splits = std::min(splits, tiles / pl.min_tiles);
     pl.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(splits, kMaxSplits)));
     if (pl.splits > 1)
         pl.workspace = static_cast<uint64_t>(tokens) * a->num_heads * pl.splits * (a->head_dim + 2) * 4;
@@ -187,6 +193,7 @@ int kvx_paged_attention(int32_t device, const kvx_attention* args, void* workspa
     p.window = a.window > 0 ? a.window : INT_MAX;
     p.sinks = a.sinks;
     p.splits = pl.splits;
+    p.min_tiles = pl.min_tiles;
     p.tile_tokens = pl.tile_tokens;
     p.tile_slots = pl.tile_slots;
     p.out_wide = ((a.out | static_cast<uint64_t>(a.out_token_stride) | static_cast<uint64_t>(a.out_head_stride)) & 31) == 0;
@@ -194,6 +201,8 @@ int kvx_paged_attention(int32_t device, const kvx_attention* args, void* workspa
         p.ws_o = static_cast<float*>(workspace_dev);
         p.ws_ml = p.ws_o + static_cast<int64_t>(a.num_tokens) * a.num_heads * pl.splits * a.head_dim;
     }
+    if (pl.splits > 1 && static_cast<int64_t>(a.num_tokens) * a.num_heads > INT_MAX)
+        return fail(KVX_EINVAL, "num_tokens * num_heads is beyond 2^31");
     KVX_DEVICE_GUARD(device);
     const auto st = static_cast<cudaStream_t>(stream);
     const bool q4 = a.cache_bits == 4;

@@ -42,7 +42,7 @@ struct AttnParams {
     int32_t num_seqs, num_tokens;
     int32_t heads, kv_heads, group;
     int32_t window, sinks;                    // window: INT_MAX when there is none
-    int32_t splits;
+    int32_t splits, min_tiles;                // key tiles of a split, at least
     int32_t tile_tokens;                      // tokens of an item
     int32_t tile_slots;                       // item slots per (kv head, split)
     int32_t out_wide;                         // output rows start at multiples of 32 bytes
@@ -134,7 +134,8 @@ __device__ __forceinline__ KeyTiles key_tiles(const AttnParams& p, const AttnIte
     t.head = min(sink_tiles, low_tile);
     t.skip = low_tile - t.head;
     const int n = total - t.skip;
-    const int per = (n + p.splits - 1) / p.splits;
+    // A split of its own only for enough keys: the host knows no lengths, only what a table can hold.
+    const int per = max((n + p.splits - 1) / p.splits, p.min_tiles);
     t.begin = min(n, it.split * per);
     t.end = min(n, t.begin + per);
     return t;
@@ -301,7 +302,7 @@ __device__ __noinline__ void visible_scores(const AttnParams& p, const AttnItem&
 // Launches (one translation unit per kernel family)
 // ---------------------------------------------------------------------------
 
-// Rows are few: keys split over CTAs and warps (kvx_attn_split.cu). An item has 8 * nt rows (nt = 1 to 4).
+// Rows are few: keys split over CTAs and warps (kvx_attn_split.cu). An item has 8 * nt rows (nt = 1 to 3).
 int launch_attn_split(const AttnParams& p, int head_dim, int dtype, bool q4, int nt, int device, cudaStream_t stream);
 // Rows are many: 256-row tiles on the tensor cores (kvx_attn_tile.cu).
 int launch_attn_tile(const AttnParams& p, int head_dim, int dtype, bool q4, int device, int sms, cudaStream_t stream);

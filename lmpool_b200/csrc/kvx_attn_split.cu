@@ -132,6 +132,14 @@ __global__ void __launch_bounds__(kSplitWarps * 32, Q4 && NT == 1 ? 4 : 2) attn_
     if (it.tokens == 0) return;
     const KeyTiles kt = key_tiles<C::kKeys>(p, it);
     const int rows = it.tokens * p.group;
+    if (kt.begin == kt.end && p.splits > 1) {                      // a split without keys: the join reads no more of it
+        for (int row = threadIdx.x; row < rows; row += kSplitWarps * 32) {
+            const int64_t at = (static_cast<int64_t>(it.q0 + row / p.group) * p.heads + it.head * p.group + row % p.group) *
+                                   p.splits + it.split;
+            *reinterpret_cast<float2*>(p.ws_ml + at * 2) = make_float2(-INFINITY, 0.f);
+        }
+        return;
+    }
     const int32_t* table = p.table + it.seq * p.table_stride;
     const int last = it.pos0 + it.tokens - 1;
     const int64_t head_off = it.head * p.head_stride;
@@ -632,6 +640,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const __grid
     const float* o = p.ws_o + row * p.splits * D + lane * N;
 #pragma unroll 8
     for (int i = warp; i < p.splits; i += kJoinWarps) {
+        const float f = weight[i];
+        if (f == 0.f) continue;
         float v[N];
         if constexpr (N == 4) {
             const float4 w = __ldcg(reinterpret_cast<const float4*>(o + static_cast<int64_t>(i) * D));
@@ -640,10 +650,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const __grid
             const float2 w = __ldcg(reinterpret_cast<const float2*>(o + static_cast<int64_t>(i) * D));
             v[0] = w.x, v[1] = w.y;
         }
-        const float f = weight[i];
 #pragma unroll
-        for (int k = 0; k < N; ++k)
-            if (f != 0.f) acc[k] = fmaf(f, v[k], acc[k]);
+        for (int k = 0; k < N; ++k) acc[k] = fmaf(f, v[k], acc[k]);
     }
 #pragma unroll
     for (int k = 0; k < N; ++k) part[warp][lane * N + k] = acc[k];
@@ -714,8 +722,7 @@ static int run_rows(const AttnParams& p, int nt, int device, cudaStream_t stream
     switch (nt) {
         case 1: return run_split<T, D, 1, Q4>(p, device, stream);
         case 2: return run_split<T, D, 2, Q4>(p, device, stream);
-        case 3: return run_split<T, D, 3, Q4>(p, device, stream);
-        default: return run_split<T, D, 4, Q4>(p, device, stream);
+        default: return run_split<T, D, 3, Q4>(p, device, stream);
     }
 }
 

@@ -610,7 +610,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                 const int64_t at =
                     (static_cast<int64_t>(it.q0 + token) * p.heads + it.head * p.group + head) * p.splits + it.split;
                 char* dst = p.out + (it.q0 + token) * p.o_token_stride + (it.head * p.group + head) * p.o_head_stride;
-                if (n <= 0 && live && p.splits > 1) *reinterpret_cast<float2*>(p.ws_ml + at * 2) = make_float2(-INFINITY, 0.f);
+                if (n <= 0 && p.splits > 1) {                       // a split without keys: the join reads no more of it
+                    if (live) *reinterpret_cast<float2*>(p.ws_ml + at * 2) = make_float2(-INFINITY, 0.f);
+                    continue;
+                }
                 bool nan = false;
 #pragma unroll 1
                 for (int c = 0; c < D; c += 16) {

@@ -1,6 +1,10 @@
 """CPU tests of the 4-bit cache's definition and of the refusals that need no GPU."""
 import ctypes
 import math
+import shutil
+import struct
+import subprocess
+from pathlib import Path
 
 import pytest
 import torch
@@ -65,6 +69,31 @@ def test_attention_refuses_before_touching_a_gpu(kvx_lib, bad):
     status = ctypes.c_int32(0)
     rc = kvx_lib.kvx_paged_attention(0, _args(**bad), None, 0, ctypes.addressof(status), None)
     assert rc == _capi.KVX_EINVAL and kvx_lib.kvx_last_error()
+
+
+def test_the_packed_struct_is_the_headers(kvx_lib, tmp_path):
+    """pack_attention writes kvx_attention field by field: same size, same places."""
+    src = tmp_path / "layout.c"
+    src.write_text("""
+#include <stdio.h>
+#include "kvx.h"
+int main(void) {
+    printf("%zu %zu %zu %zu %zu %zu\\n", sizeof(kvx_attention), offsetof(kvx_attention, cu_seqlens_q),
+           offsetof(kvx_attention, num_blocks), offsetof(kvx_attention, num_tokens), offsetof(kvx_attention, sinks),
+           offsetof(kvx_attention, v_scale));
+    return 0;
+}
+""")
+    if shutil.which("gcc") is None:
+        pytest.skip("gcc not installed")
+    root = Path(__file__).resolve().parent.parent
+    subprocess.run(["gcc", "-std=c11", "-Wall", "-Werror", "-I", str(root / "include"), str(src), "-o", str(tmp_path / "l")],
+                   check=True, capture_output=True)
+    got = [int(x) for x in subprocess.run([str(tmp_path / "l")], capture_output=True, text=True, check=True).stdout.split()]
+    at_of = lambda n: struct.calcsize("=" + n)  # noqa: E731
+    assert got == [struct.calcsize("=7Q9q11i3f2i"), at_of("6Q"), at_of("7Q8q"), at_of("7Q9q"), at_of("7Q9q10i"),
+                   at_of("7Q9q11i2f")]
+    assert len(_args()) == got[0]
 
 
 def test_attention_needs_a_status_word(kvx_lib):

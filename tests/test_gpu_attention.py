@@ -325,6 +325,47 @@ def test_query_strides_and_given_output(require_gpu, q4):
     assert torch.equal(f(odd, case.k, case.v, case.tables.to(DEV), case.ctx.to(DEV), 16), want)
 
 
+@pytest.mark.parametrize("q_lens", [None, [40, 70]], ids=["decode", "prompt"])
+def test_dimensions_of_one_entry_may_have_any_stride(require_gpu, q_lens):
+    """One kv head, one page, one token a page: the stride of such a dimension means nothing."""
+    for ctx, page, pages in (([40, 90], 16, None), ([40, 90], 1, None), ([40, 90], 96, 1)):
+        case = Case(ctx, 4, 1, 64, page, torch.bfloat16, False, q_lens=q_lens, seed=8)
+        if pages == 1:                      # both sequences on the same page
+            case.k, case.v, case.tables = case.k[:1].clone(), case.v[:1].clone(), torch.zeros(2, 1, dtype=torch.int32)
+        want = case.check()
+        shape, size = case.k.shape, case.k.numel()
+        odd = [1 if n == 1 else st for n, st in zip(shape, case.k.stride())]
+        f = lambda x: torch.as_strided(x.clone(), shape, odd)  # noqa: E731
+        assert f(case.k).numel() == size
+        got = at.paged_attention(case.q.to(DEV), f(case.k), f(case.v), case.tables.to(DEV), case.ctx.to(DEV), page,
+                                 cu_seqlens_q=None if case.cu is None else case.cu.to(DEV))
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype,q4", TYPES, ids=IDS)
+@pytest.mark.parametrize("q_len", [0, 5, 40])
+def test_short_contexts_in_wide_tables(require_gpu, dtype, q4, q_len):
+    """Tables wide enough for long contexts: most splits have no keys."""
+    ctx = [40, 3, 700]
+    case = Case(ctx, 4, 1, 64, 16, dtype, q4, q_lens=[min(q_len, c) for c in ctx] if q_len else None, seed=15)
+    case.tables = torch.cat((case.tables, torch.full((3, 3000), -1, dtype=torch.int32)), 1)
+    case.check()
+    case.check(window=9, sinks=1)
+
+
+@pytest.mark.parametrize("q4", [False, True])
+@pytest.mark.parametrize("most", [3, 60])
+def test_many_ragged_sequences(require_gpu, q4, most):
+    """More sequences than a warp has lanes, many of them without tokens, some without a context."""
+    rng = random.Random(most)
+    ctx = [rng.choice([0, 1, rng.randint(1, 60), rng.randint(1, 200)]) for _ in range(75)]
+    q_lens = [min(c, rng.choice([0, 1, rng.randint(0, most)])) for c in ctx]
+    q_lens[40] = most                                   # more tokens than its context may hold
+    case = Case(ctx, 4, 2, 64, 16, torch.float16, q4, q_lens=q_lens, seed=16)
+    case.check()
+    case.check(window=11, sinks=2)
+
+
 def test_cache_orders(require_gpu):
     """A cache whose heads lie before its slots, and one layer of a stacked cache."""
     case = Case([40, 90], 4, 2, 64, 16, torch.float16, False, seed=8)
@@ -575,6 +616,8 @@ def test_refusals(require_gpu):
         call(scale=float("nan"))
     with pytest.raises(RuntimeError):
         call(out=torch.empty(2, 4, 64, dtype=torch.bfloat16, device=DEV))
+    with pytest.raises(RuntimeError, match="out must not"):
+        call(out=q)
     with pytest.raises(RuntimeError, match="CUDA"):
         call(q=q.cpu(), k=k.cpu(), v=v.cpu(), table=table.cpu(), ctx=ctx.cpu())
     with pytest.raises(RuntimeError):
