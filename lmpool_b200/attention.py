@@ -171,27 +171,40 @@ def q4_row_bytes(head_dim: int) -> int:
     return head_dim // 2 + head_dim // 16
 
 
-def _q4_check(k_cache: torch.Tensor, v_cache: torch.Tensor, block_size: int, head_dim: int) -> None:
+def _q4_check(k_cache: torch.Tensor, v_cache: torch.Tensor, block_size: int, head_dim: int) -> int:
+    """Checks a 4-bit cache; its block stride in bytes."""
     if k_cache.dtype != torch.uint8 or v_cache.dtype != torch.uint8:
         raise TypeError("a 4-bit cache holds bytes: k_cache and v_cache must be uint8")
-    if k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride():
+    shape, st = k_cache.shape, k_cache.stride()
+    if shape != v_cache.shape or st != v_cache.stride():
         raise RuntimeError("k_cache and v_cache must have the same shape and strides")
-    if k_cache.dim() != 4:
+    if len(shape) != 4:
         raise RuntimeError("k_cache must be [num_blocks, block_size, num_kv_heads, head_dim / 2 + head_dim / 16]")
-    _, bs, H, row = k_cache.shape
-    if bs != block_size or row != q4_row_bytes(head_dim):
+    N, bs, H, row = shape
+    if bs != block_size or row * 16 != head_dim * 9 or head_dim % 16:
         raise RuntimeError(f"a 4-bit cache for block_size {block_size} and head_dim {head_dim} is [num_blocks, "
-                           f"{block_size}, num_kv_heads, {q4_row_bytes(head_dim)}], got {list(k_cache.shape)}")
-    st = k_cache.stride()
+                           f"{block_size}, num_kv_heads, head_dim / 2 + head_dim / 16], got {list(shape)}")
     if st[3] != 1 or (H > 1 and st[2] != row) or (bs > 1 and st[1] != H * row):
         raise RuntimeError("each page [block_size, num_kv_heads, row] of a 4-bit cache must be contiguous")
+    return st[0] if N > 1 else bs * H * row
+
+
+def _same_device(first: torch.Tensor, *others: torch.Tensor) -> int:
+    """The CUDA device of all of them (raises as ``_device_of``, at less cost a call)."""
+    device = first.get_device()
+    if device < 0:
+        return _device_of(first, *others)
+    for t in others:
+        if t.get_device() != device:
+            return _device_of(first, *others)
+    return device
 
 
 def _rows_of(x: torch.Tensor) -> torch.Tensor:
-    """x [T, H, D] with contiguous, 16-byte aligned token rows (a copy where it has none)."""
-    T, H, D = x.shape
+    """16-bit x [T, H, D] with contiguous, 16-byte aligned token rows (a copy where it has none)."""
+    _, H, D = x.shape
     st = x.stride()
-    if st[2] == 1 and (H == 1 or st[1] == D) and st[0] * x.element_size() % 16 == 0 and x.data_ptr() % 16 == 0:
+    if st[2] == 1 and (H == 1 or st[1] == D) and st[0] % 8 == 0 and x.data_ptr() % 16 == 0:
         return x
     return x.contiguous() if not x.is_contiguous() else x.clone()
 
@@ -227,19 +240,19 @@ def store_kvcache_q4(
     if key.dtype not in _DTYPE_CODE or value.dtype != key.dtype:
         raise TypeError(f"key and value must both be bfloat16 or float16, got {key.dtype} and {value.dtype}")
     assert slot_mapping.numel() == T, "Slot mapping size must match number of tokens"
-    _q4_check(k_cache, v_cache, block_size, D)
-    if k_cache.shape[2] != H:
+    block_stride = _q4_check(k_cache, v_cache, block_size, D)
+    num_blocks, _, kv_heads, _ = k_cache.shape
+    if kv_heads != H:
         raise RuntimeError("key/value [T, H, D] must match the cache's kv heads")
     slot_mapping = _check_slots(slot_mapping)
-    device = _device_of(key, value, k_cache, v_cache, slot_mapping)
+    device = _same_device(key, value, k_cache, v_cache, slot_mapping)
     if T == 0:
         return
     key, value = _rows_of(key), _rows_of(value)
     rc = _capi.lib().kvx_store_kvcache_q4(
         device, _DTYPE_CODE[key.dtype], key.data_ptr(), value.data_ptr(), key.stride(0) * 2, value.stride(0) * 2,
-        k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0) if k_cache.shape[0] > 1 else 0, slot_mapping.data_ptr(), T,
-        k_cache.shape[0],
-        int(block_size), H, D, k_scale, v_scale, _status(device), _raw_stream(device))
+        k_cache.data_ptr(), v_cache.data_ptr(), block_stride, slot_mapping.data_ptr(), T, num_blocks, block_size, H, D,
+        k_scale, v_scale, _status(device), _raw_stream(device))
     if rc:
         _capi.check(rc, "kvx_store_kvcache_q4")
 
@@ -261,9 +274,9 @@ def load_kvcache_q4(
     if k_cache.dim() != 4 or k_cache.shape[3] % 9:
         raise RuntimeError("k_cache must be [num_blocks, block_size, num_kv_heads, head_dim / 2 + head_dim / 16]")
     D = k_cache.shape[3] // 9 * 16
-    _q4_check(k_cache, v_cache, block_size, D)
+    block_stride = _q4_check(k_cache, v_cache, block_size, D)
     slot_mapping = _check_slots(slot_mapping)
-    device = _device_of(k_cache, v_cache, slot_mapping)
+    device = _same_device(k_cache, v_cache, slot_mapping)
     T, H = slot_mapping.numel(), k_cache.shape[2]
     key = torch.empty((T, H, D), dtype=dtype, device=k_cache.device)
     value = torch.empty_like(key)
@@ -271,8 +284,7 @@ def load_kvcache_q4(
         return key, value
     rc = _capi.lib().kvx_load_kvcache_q4(
         device, _DTYPE_CODE[dtype], key.data_ptr(), value.data_ptr(), H * D * 2, H * D * 2, k_cache.data_ptr(),
-        v_cache.data_ptr(), k_cache.stride(0) if k_cache.shape[0] > 1 else 0, slot_mapping.data_ptr(), T, k_cache.shape[0],
-        int(block_size), H, D,
+        v_cache.data_ptr(), block_stride, slot_mapping.data_ptr(), T, k_cache.shape[0], block_size, H, D,
         k_scale, v_scale, _status(device), _raw_stream(device))
     if rc:
         _capi.check(rc, "kvx_load_kvcache_q4")
@@ -306,8 +318,7 @@ def _paged_attention(query, k_cache, v_cache, block_tables, context_lens, block_
         raise RuntimeError(f"head_dim must be 64 or 128, got {D}")
     st = k_cache.stride()
     if bits == 4:
-        _q4_check(k_cache, v_cache, block_size, D)
-        block_stride, slot_stride, head_stride = st[0] if k_cache.shape[0] > 1 else 0, 0, 0
+        block_stride, slot_stride, head_stride = _q4_check(k_cache, v_cache, block_size, D), 0, 0
     else:
         if k_cache.dtype != dtype or v_cache.dtype != dtype:
             raise TypeError("query and cache dtypes must match")
@@ -339,10 +350,7 @@ def _paged_attention(query, k_cache, v_cache, block_tables, context_lens, block_
         table_stride = width
     if S > 1 and context_lens.stride(0) != 1:
         context_lens = context_lens.contiguous()
-    device = query.get_device()
-    if device < 0 or device != k_cache.get_device() or device != v_cache.get_device() \
-            or device != block_tables.get_device() or device != context_lens.get_device():
-        _device_of(query, k_cache, v_cache, block_tables, context_lens)      # says which
+    device = _same_device(query, k_cache, v_cache, block_tables, context_lens)
     cu = 0
     if cu_seqlens_q is None:
         if T != S:
@@ -354,7 +362,7 @@ def _paged_attention(query, k_cache, v_cache, block_tables, context_lens, block_
             raise RuntimeError(f"cu_seqlens_q must hold num_seqs + 1 = {S + 1} entries")
         if S > 0 and cu_seqlens_q.stride(0) != 1:
             cu_seqlens_q = cu_seqlens_q.contiguous()
-        _device_of(query, cu_seqlens_q)
+        _same_device(query, cu_seqlens_q)
         cu = cu_seqlens_q.data_ptr()
     if window is None:
         window = 0
@@ -372,7 +380,7 @@ def _paged_attention(query, k_cache, v_cache, block_tables, context_lens, block_
     else:
         if out.shape != query.shape or out.dtype != dtype:
             raise RuntimeError("out must have query's shape and dtype")
-        _device_of(query, out)
+        _same_device(query, out)
         os = out.stride()
         if os[2] != 1 or os[0] % 8 or os[1] % 8 or out.data_ptr() % 16:
             raise RuntimeError("out must have contiguous, 16-byte aligned rows of head_dim")
