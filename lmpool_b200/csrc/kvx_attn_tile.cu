@@ -458,25 +458,36 @@ __device__ __forceinline__ void issue_copies(const AttnParams& p, const TileMaps
         const int n = kt.end - kt.begin;
         const int last = it.pos0 + it.tokens - 1;
         const int32_t* table = p.table + it.seq * p.table_stride;
+        // This lane's page of a tile, if some row sees its keys. On a 4-bit cache it is read while the tile before is
+        // copied (five drafted tokens of 32 sequences, window 2048: 102 us, 109 without); a 16-bit ring has more in
+        // flight and gains nothing by it (256 sequences of 600 keys: 168 us, 176 with).
+        bool wanted = false;
+        int id = -1, slot = 0;
+        auto look_up = [&](int tile) {
+            const int j = kt.first_key<kTileKeys>(kt.begin + tile) + at;
+            wanted = run > 0 && tile < n && at < kTileKeys && j <= last && (it.pos0 - (j + run - 1) < p.window || j < p.sinks);
+            id = -1;
+            if (wanted) {
+                const int blk = block_of(p, j);
+                slot = j - blk * p.block_size;
+                if (blk < p.table_width) id = table[blk];
+            }
+        };
+        if (Q4) look_up(0);
         for (int op = 0; op < 2 * n; ++op, ring.next()) {
-            const int j = kt.first_key<kTileKeys>(kt.begin + (op >> 1)) + at;
             if constexpr (!Q4) {
                 if (!warp_wait(&bars->empty[ring.at], ring.phase ^ 1, abort, p.status)) return;
-                if (run == 0 || gathered(run, op, j - at, last)) {
+                if (run == 0 || gathered(run, op, kt.first_key<kTileKeys>(kt.begin + (op >> 1)), last)) {
                     if (lane == 0) mbar_arrive(&bars->full[ring.at]);
                     continue;
                 }
+                if (!(op & 1)) look_up(op >> 1);
             }
-            // Keys that some row sees, in a page that exists.
-            int id = -1, slot = 0;
-            if (at < kTileKeys && j <= last && (it.pos0 - (j + run - 1) < p.window || j < p.sinks)) {
-                const int blk = block_of(p, j);
-                slot = j - blk * p.block_size;
-                id = blk < p.table_width ? table[blk] : -1;
-                if (id < 0 || id >= p.num_blocks) {
-                    atomicOr(p.status, KVX_DEV_BAD_SRC_ID);
-                    id = -1;
-                }
+            if constexpr (Q4)
+                if (!warp_wait(&bars->raw_empty[ring.at], ring.phase ^ 1, abort, p.status)) return;
+            if (wanted && (id < 0 || id >= p.num_blocks)) {
+                atomicOr(p.status, KVX_DEV_BAD_SRC_ID);
+                id = -1;
             }
             if constexpr (!Q4) {
                 uint64_t* bar = &bars->full[ring.at];
@@ -490,7 +501,6 @@ __device__ __forceinline__ void issue_copies(const AttnParams& p, const TileMaps
                         tma_load4(tile + c * C::kSlabBytes + at * 128, op & 1 ? &maps.v : &maps.k, 64 * c, slot, it.head,
                                   id < 0 ? static_cast<int>(p.num_blocks) : id, bar);
             } else {
-                if (!warp_wait(&bars->raw_empty[ring.at], ring.phase ^ 1, abort, p.status)) return;
                 uint64_t* bar = &bars->raw_full[ring.at];
                 const uint32_t take = __ballot_sync(~0u, id >= 0);
                 if (lane == 0) {
@@ -506,6 +516,7 @@ __device__ __forceinline__ void issue_copies(const AttnParams& p, const TileMaps
                              16 * (D / 16), bar);
                 }
             }
+            if (Q4 && (op & 1)) look_up((op >> 1) + 1);
         }
     }
 }
