@@ -3,7 +3,8 @@
 Modules:
   kv_transfer   drop-in for lmpool.engine.kv_transfer (pack/unpack, swap_in,
                 swap_out, prewarm_p2p_pairs) plus move_blocks / swap_batch
-  attention     drop-in store_kvcache (+ all-layer variant)
+  attention     drop-in store_kvcache (+ all-layer variant); 4-bit KV cache
+                (store/load) and attention over paged 16-bit and 4-bit caches
   model_runner  ModelRunner transfer boundary (execute_swap_out/in,
                 kv_transfer_bytes)
   endpoint      per-GPU mailbox, peer mappings, pair protocol

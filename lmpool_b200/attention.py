@@ -384,6 +384,8 @@ def _paged_attention(query, k_cache, v_cache, block_tables, context_lens, block_
         os = out.stride()
         if os[2] != 1 or os[0] % 8 or os[1] % 8 or out.data_ptr() % 16:
             raise RuntimeError("out must have contiguous, 16-byte aligned rows of head_dim")
+        if (heads > 1 and os[1] < D) or (T > 1 and os[0] < D):
+            raise RuntimeError("out's rows must not overlap")
         if out.data_ptr() == query.data_ptr() and T:
             raise RuntimeError("out must not be the query")
     if T == 0 or S == 0:
@@ -436,7 +438,8 @@ def paged_attention(
     from 0) sequence ``s`` has the tokens ``cu_seqlens_q[s]`` to ``cu_seqlens_q[s + 1]``, the last of its context:
     prompts, chunks of prompts, drafted tokens. Token at position ``p`` sees key ``j <= p`` if ``window`` is None, if
     ``p - j < window`` or if ``j < sinks``. A token that sees no key gets zeros. Rows behind the last sequence are left
-    as they were. ``out`` takes the result and must not overlap the inputs. ``scale`` (default ``D ** -0.5``) must be positive.
+    as they were. ``out`` takes the result and must not overlap the inputs. ``scale`` (default ``D ** -0.5``) must be
+    positive. No gradient is recorded: this reads a serving cache.
 
     Runs on the current stream without synchronising; lengths and tables are read on the device, so a captured call
     can be replayed with others. Bad page ids (their keys read as zeros) and lengths are recorded in the device's

@@ -70,8 +70,8 @@ static int check_args(const kvx_attention* a) {
     return KVX_OK;
 }
 
-// `sms` fills the GPU: 2 CTAs of the split kernel fit an SM on a 16-bit cache
-// (shared memory), 4 on a 4-bit one (registers); the tile kernel has one.
+// What fills the GPU: an SM takes 2 CTAs of the split kernel on a 16-bit cache (shared memory), 4 on a 4-bit one with
+// one row tile, 2 with more (registers); the tile kernel has one.
 static AttnPlan plan_of(const kvx_attention* a, int sms) {
     AttnPlan pl{};
     const int group = a->num_heads / a->num_kv_heads;

@@ -653,3 +653,15 @@ def test_refusals(require_gpu):
         at.load_kvcache_q4(kc, kc, slots, 16, dtype=torch.float32)
     torch.cuda.synchronize()
     kt.check_device_status(0)
+
+
+@pytest.mark.gpu
+def test_an_output_whose_rows_share_memory_is_refused(require_gpu):
+    q = torch.zeros(2, 4, 64, dtype=torch.bfloat16, device=DEV)
+    cache = torch.zeros(2, 16, 2, 64, dtype=torch.bfloat16, device=DEV)
+    tables = torch.zeros(2, 1, dtype=torch.int32, device=DEV)
+    ctx = torch.ones(2, dtype=torch.int32, device=DEV)
+    for out in (torch.empty(1, 4, 64, dtype=torch.bfloat16, device=DEV).expand(2, 4, 64),
+                torch.empty(2, 1, 64, dtype=torch.bfloat16, device=DEV).expand(2, 4, 64)):
+        with pytest.raises(RuntimeError, match="must not overlap"):
+            at.paged_attention(q, cache, cache.clone(), tables, ctx, 16, out=out)
