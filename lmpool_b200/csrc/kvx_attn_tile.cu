@@ -809,11 +809,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
         int my_token[2], my_head[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int row = 64 * w + 32 * h + lane;
+            const int row = kHalfRows * h + 32 * w + lane;
             my_token[h] = row / p.group;
             my_head[h] = row - my_token[h] * p.group;
         }
-        bool ok = true;
+        bool ok = true, fresh = true;
         Ring<kWork> work;
         while (ok) {
             AttnItem it;
@@ -822,24 +822,30 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
             const int n = kt.end - kt.begin;
             if (n <= 0) continue;
             const int last = it.pos0 + it.tokens - 1;
-            const int q_after = n > 1 ? 3 : 2;                      // the queries follow this many key and value tiles
+            // The queries follow this many key and value tiles of the item. (The first item's come before them: nothing
+            // is in their place yet, and no product can start without them.)
+            const int q_after = fresh ? 0 : n > 1 ? 3 : 2;
+            fresh = false;
+            const int row_tiles = second_tile(p, it) ? 2 : 1;
             for (int op = 0; op <= 2 * n; ++op) {
                 if (op == q_after) {
                     if (!(ok = warp_wait(&bars->q_empty, q_phase, abort, p.status))) break;
                     q_phase ^= 1;
-                    int64_t off[2];                                 // of rows 64 w + lane and 32 further
+                    int64_t off[2];                                 // of this lane's row of each row tile
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
                         off[h] = my_token[h] < it.tokens ? (it.q0 + my_token[h]) * p.q_token_stride +
                                                                (it.head * p.group + my_head[h]) * p.q_head_stride
                                                          : -1;
+#pragma unroll 1
+                    for (int h = 0; h < row_tiles; ++h) {
+                        const int64_t mine = h ? off[1] : off[0];
 #pragma unroll 4
-                    for (int s = 0; s < 64; s += kRowsPerStep) {
-                        const int row = 64 * w + s + lane / kChunks, c = lane % kChunks;
-                        const int64_t from = __shfl_sync(~0u, s < 32 ? off[0] : off[1], row & 31);
-                        const bool take = from >= 0;
-                        const char* src = p.q + 16 * c + (take ? from : 0);
-                        cp16(chunk_at(base + (row >> 7) * C::kTileBytes, row & 127, c), src, take);
+                        for (int s = 0; s < 32; s += kRowsPerStep) {
+                            const int r = s + lane / kChunks, c = lane % kChunks;
+                            const int64_t from = __shfl_sync(~0u, mine, r);
+                            cp16(chunk_at(base + h * C::kTileBytes, 32 * w + r, c), p.q + 16 * c + (from >= 0 ? from : 0), from >= 0);
+                        }
                     }
                     asm volatile("cp.async.wait_all;" ::: "memory");
                     if constexpr (Q4 && !std::is_same<T, __half>::value) {
@@ -847,9 +853,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                         // ordered as numbers), then the elements over its power of two.
                         __syncwarp();
 #pragma unroll 1
-                        for (int s = 0; s < 64; s += 32) {
-                            const int row = 64 * w + s + lane;
-                            const uint32_t tile = base + (row >> 7) * C::kTileBytes;
+                        for (int h = 0; h < row_tiles; ++h) {
+                            const int row = kHalfRows * h + 32 * w + lane;
+                            if (__all_sync(~0u, (h ? my_token[1] : my_token[0]) >= it.tokens)) {
+                                factors[row] = 1.f;                 // no rows here: zeros already
+                                continue;
+                            }
+                            const uint32_t tile = base + h * C::kTileBytes;
                             uint32_t big = 0;
 #pragma unroll 4
                             for (int c = 0; c < kChunks; ++c) {
@@ -872,7 +882,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                             }
                         }
                     } else if constexpr (Q4) {
-                        for (int s = 0; s < 64; s += 32) factors[64 * w + s + lane] = 1.f;
+                        for (int h = 0; h < 2; ++h) factors[kHalfRows * h + 32 * w + lane] = 1.f;
                     }
                     fence_async_shared();
                     mbar_arrive(&bars->q_full);
