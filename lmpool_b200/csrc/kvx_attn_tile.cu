@@ -40,6 +40,12 @@
 // 1/2, on the FMA units, with a degree-4 polynomial (relative error 2.8e-6, from a
 // weighted least-squares fit of 2^f; the weights are rounded to 2^-8 or 2^-11).
 //
+// Measured: a prompt of 8191 tokens, window 1024, 32 query heads on 8: 205 us (76 us of products at the rate of a large
+// library product); 4 prompts of 129 to 4095 tokens on up to 2001 earlier ones: 441 us (218 us); two of 3001 to 4096 on a
+// 4-bit cache: 391 us (183 us). A key tile takes two row tiles about 4200 clocks, of which the tensor cores are busy 2560:
+// the rest is issue slots, which the exponentials of 8 warps and the issuing of products share (more code or state
+// in either loop costs at once: two more values kept in the softmax loop, 4 %).
+//
 // Every wait is bounded: where one runs out, the CTA flags KVX_DEV_PIPE_TIMEOUT,
 // all warps leave their loops, and tensor memory is freed.
 
