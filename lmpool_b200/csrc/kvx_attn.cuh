@@ -216,6 +216,11 @@ __device__ __forceinline__ uint32_t scales_to_half(uint32_t two) {
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
     return r;
 }
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
 // code * scale has at most six significant bits and lies in [2^-10, 2688]: exact.
 __device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
     uint32_t r;

@@ -98,35 +98,35 @@ __global__ void __launch_bounds__(kQ4Threads) store_q4_kernel(const __grid_const
     raw[0] = lo.x, raw[1] = lo.y, raw[2] = lo.z, raw[3] = lo.w;
     raw[4] = hi.x, raw[5] = hi.y, raw[6] = hi.z, raw[7] = hi.w;
     const float mul = plane ? p.v_mul : p.k_mul;
-    float x[16];
-    float amax = 0.f;
-    bool finite = true;
+    // The largest magnitude: the bits of bf16 and of fp16 without their sign are ordered as numbers, NaN above infinity.
+    uint32_t most = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float2 v = Pair<T>::unpack(raw[i]);
-        x[2 * i] = v.x * mul;
-        x[2 * i + 1] = v.y * mul;
-        finite &= fabsf(x[2 * i]) < INFINITY && fabsf(x[2 * i + 1]) < INFINITY;
-        amax = fmaxf(amax, fmaxf(fabsf(x[2 * i]), fabsf(x[2 * i + 1])));
-    }
+    for (int i = 0; i < 8; ++i) most = max_u16x2(most, raw[i] & 0x7fff7fffu);
+    most = max(most & 0xffffu, most >> 16);
+    const float amax = Pair<T>::unpack(most).x * mul;
+    const bool finite = amax < INFINITY;
     uint16_t scale2;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %1;" : "=h"(scale2) : "f"(__fdiv_rn(amax, 6.f)));
     const float s = Pair<__half>::unpack(scales_to_half(scale2)).x;
-    const float r = s > 0.f ? __frcp_rn(s) : 0.f;
-    uint32_t codes[2] = {0, 0};
+    const float r = s > 0.f ? __frcp_rn(s) * mul : 0.f;         // mul is a power of two: as exact as 1 / s
+    uint32_t codes[2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        float y[2];
+    for (int i = 0; i < 2; ++i) {
+        float y[8];
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-            y[k] = __uint_as_float((__float_as_uint(x[2 * i + k] * r) + 0x10u) & ~0x1fu);
-        uint32_t c;
-        asm("{\n\t.reg .b8 t;\n\t"
-            "cvt.rn.satfinite.e2m1x2.f32 t, %1, %2;\n\t"
-            "cvt.u32.u8 %0, t;\n\t}"
-            : "=r"(c)
-            : "f"(y[1]), "f"(y[0]));
-        codes[i >> 2] |= c << (8 * (i & 3));
+        for (int k = 0; k < 4; ++k) {
+            const float2 v = Pair<T>::unpack(raw[4 * i + k]);
+            y[2 * k] = __uint_as_float((__float_as_uint(v.x * r) + 0x10u) & ~0x1fu);
+            y[2 * k + 1] = __uint_as_float((__float_as_uint(v.y * r) + 0x10u) & ~0x1fu);
+        }
+        asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+            "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+            "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+            "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+            "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+            "mov.b32 %0, {a, b, c, d};\n\t}"
+            : "=r"(codes[i])
+            : "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7]));
     }
     if (!finite) scale2 = 0x7f;
     if (!finite || s == 0.f) codes[0] = codes[1] = 0;
