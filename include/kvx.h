@@ -342,7 +342,7 @@ int kvx_store_kvcache_layers(int32_t device, int32_t num_layers, const void* key
  * bytes, and a page is `kv_heads` such runs in a row: to the block mover it is
  * an opaque chunk, 3.56x smaller than a 16-bit one.
  * head_dim must be a multiple of 16 and at most 256, block_size a multiple of
- * 16; strides and addresses multiples of 16 bytes. dtype: 0 = bf16, 1 = fp16.
+ * 16, block_size * head_dim below 2^30; strides and addresses multiples of 16 bytes. dtype: 0 = bf16, 1 = fp16.
  * Slots as in kvx_store_kvcache: -1 is padding, others outside the cache are
  * skipped and flagged with KVX_DEV_BAD_SLOT; two tokens of one call must not
  * share a slot. kvx_load_kvcache_q4 reads rows back (code * s * k_scale,

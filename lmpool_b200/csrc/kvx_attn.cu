@@ -51,6 +51,9 @@ static int check_args(const kvx_attention* a) {
     if (a->block_size <= 0) return fail(KVX_EINVAL, "block_size must be > 0");
     if (a->cache_bits == 4 && a->block_size % 16 != 0)
         return fail(KVX_EINVAL, "block_size of a 4-bit cache must be a multiple of 16");
+    // The kernels index within a (page, head) of a 4-bit cache in 32 bits, as the store does.
+    if (a->cache_bits == 4 && static_cast<int64_t>(a->block_size) * a->head_dim > INT_MAX / 2)
+        return fail(KVX_EINVAL, "block_size * head_dim is too large");
     if (a->table_width < 0) return fail(KVX_EINVAL, "table_width must be >= 0");
     if (static_cast<int64_t>(a->table_width) * a->block_size > INT_MAX - 1024)
         return fail(KVX_EINVAL, "table_width * block_size is beyond 2^31 - 1025 keys");

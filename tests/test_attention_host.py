@@ -71,6 +71,18 @@ def test_attention_refuses_before_touching_a_gpu(kvx_lib, bad):
     assert rc == _capi.KVX_EINVAL and kvx_lib.kvx_last_error()
 
 
+@pytest.mark.parametrize("dim,bs", [(128, 1 << 25), (64, 1 << 26), (128, (1 << 23) + 16)])
+def test_4bit_pages_beyond_32_bit_offsets_are_refused(kvx_lib, dim, bs):
+    """Offsets within a (page, head) are 32-bit numbers: the store refuses such pages, and so does what reads them."""
+    status = ctypes.c_int32(0)
+    strides = [dim * 8, dim * 2, dim * 8, dim * 2, bs * dim // 16 * 9 * 2, 0, 0, 8]
+    args = _args(dim=dim, bs=bs, bits=4, width=1, strides=strides)
+    need = ctypes.c_uint64(0)
+    for rc in (kvx_lib.kvx_attention_workspace(0, args, ctypes.byref(need)),
+               kvx_lib.kvx_paged_attention(0, args, None, 0, ctypes.addressof(status), None)):
+        assert rc == _capi.KVX_EINVAL and b"too large" in kvx_lib.kvx_last_error()
+
+
 def test_the_packed_struct_is_the_headers(kvx_lib, tmp_path):
     """pack_attention writes kvx_attention field by field: same size, same places."""
     src = tmp_path / "layout.c"
