@@ -574,6 +574,100 @@ def test_random_cases(require_gpu):
 
 
 # ----------------------------------------------------------------------------------------------
+# Many items a CTA
+# ----------------------------------------------------------------------------------------------
+
+def attended64(case: Case, window=None, sinks=0) -> ref.Attended:
+    """ref.attention for sizes that a loop over rows is too slow for: the same in 64 bits, a sequence at a time."""
+    k_all, v_all = (x.to(DEV) for x in case.values())
+    q_all = case.q.to(DEV).double()
+    T, Hq, D = q_all.shape
+    H, page = k_all.shape[2], case.page
+    out, mass = torch.zeros_like(q_all), torch.zeros_like(q_all)
+    reach, keys, top = 0.0, 0, 0.0
+    cu = case.cu.tolist() if case.cu is not None else list(range(len(case.ctx) + 1))
+    for s, c in enumerate(case.ctx.tolist()):
+        n = cu[s + 1] - cu[s]
+        if n == 0 or c == 0:
+            continue
+        j = torch.arange(c)
+        blocks, offs = case.tables[s].long()[j // page].to(DEV), (j % page).to(DEV)
+        k, v = k_all[blocks, offs].permute(1, 0, 2)[:, None], v_all[blocks, offs].permute(1, 0, 2)[:, None]   # [H, 1, c, D]
+        step = max(1, (1 << 26) // (Hq * c))
+        for a in range(0, n, step):
+            b = min(n, a + step)
+            rows = slice(cu[s] + a, cu[s] + b)
+            q = q_all[rows].unflatten(1, (H, -1)).permute(1, 2, 0, 3)                                          # [H, G, b - a, D]
+            p = torch.arange(c - n + a, c - n + b, device=DEV)[:, None]
+            at_key = torch.arange(c, device=DEV)
+            seen = at_key <= p
+            if window is not None:
+                seen &= (p - at_key < window) | (at_key < sinks)
+            score = (q @ k.transpose(-1, -2)) * D ** -0.5
+            size = (q.abs() @ k.abs().transpose(-1, -2)) * D ** -0.5
+            reach = max(reach, size.masked_fill(~seen, 0.0).amax().item())
+            keys = max(keys, int(seen.sum(-1).max()))
+            w = torch.softmax(score.masked_fill(~seen, -math.inf), -1).nan_to_num(0.0)
+            out[rows] = (w @ v).permute(2, 0, 1, 3).flatten(1, 2)
+            mass[rows] = (w @ v.abs()).permute(2, 0, 1, 3).flatten(1, 2)
+        top = max(top, v.abs().max().item())
+    return ref.Attended(out.cpu(), mass.cpu(), reach, keys, top)
+
+
+def check64(case: Case, **kw) -> torch.Tensor:
+    got = case.call(**kw)
+    kt.check_device_status(0)
+    want = attended64(case, **kw)
+    err, lim = (got.cpu().double() - want.out).abs(), bound(want, case.dtype, case.q4, case.dim)
+    worst = (err / lim.clamp(min=1e-30)).max().item()
+    assert not err.isnan().any() and (err <= lim).all(), f"worst error is {worst:.3g} of its bound"
+    return got
+
+
+def items_a_cta(q_lens, group, kv_heads):
+    """Items per CTA of the kernel for many rows (a persistent CTA per SM), which takes calls of more rows a sequence
+    than either crossover."""
+    rows = -(-sum(q_lens) // len(q_lens)) * group
+    assert rows > 24
+    tokens = (128 if rows <= 128 else 256) // group
+    return sum(-(-q // tokens) for q in q_lens) * kv_heads / torch.cuda.get_device_properties(0).multi_processor_count
+
+
+@pytest.mark.parametrize("dtype,q4", TYPES, ids=IDS)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (70, 3)])
+@pytest.mark.parametrize("q_of", [(0, 1, 5, 31, 32, 33, 64, 65, 130), (1, 2, 9, 17, 32, 33)], ids=["two-tiles", "one-tile"])
+def test_many_items_with_keys_on_each_cta(require_gpu, dtype, q4, dim, window, sinks, q_of):
+    """Each persistent CTA takes many items in a row: items of one row tile and of two, of one key tile and of several,
+    without keys and without tokens in any order; more sequences than a warp has lanes."""
+    rng = random.Random(dim + len(q_of))
+    q_lens = [rng.choice(q_of) for _ in range(150)]
+    ctx = [0 if rng.random() < 0.05 else max(0, q + rng.choice((0, 0, -3, 3, 90, 300))) for q in q_lens]
+    case = Case(ctx, 32, 8, dim, 16, dtype, q4, q_lens=q_lens, seed=17)
+    assert items_a_cta(q_lens, 4, 8) > 6
+    first = check64(case, window=window, sinks=sinks)
+    assert torch.equal(first, case.call(window=window, sinks=sinks))
+
+
+@pytest.mark.parametrize("dtype,q4", TYPES, ids=IDS)
+@pytest.mark.parametrize("window,sinks", [(None, 0), (1000, 5)])
+def test_long_prompts(require_gpu, dtype, q4, window, sinks):
+    q_lens = [3001, 700, 1]
+    case = Case([3001, 2111, 1500], 16, 4, 128, 64, dtype, q4, q_lens=q_lens, seed=18)
+    check64(case, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("dtype,q4", TYPES, ids=IDS)
+def test_chunks_whose_keys_are_split(require_gpu, dtype, q4):
+    """Few items and long contexts: the key axis of the kernel for many rows is split too."""
+    for dim, group, q_lens, ctx in ((128, 4, [40, 100], [5000, 2900]), (64, 1, [70, 3], [4000, 3])):
+        case = Case(ctx, group, 1, dim, 16, dtype, q4, q_lens=q_lens, seed=dim)
+        assert -(-sum(q_lens) // 2) * group > 24
+        check64(case)
+        check64(case, window=2500, sinks=130)
+
+
+# ----------------------------------------------------------------------------------------------
 # Refusals
 # ----------------------------------------------------------------------------------------------
 
