@@ -369,6 +369,9 @@ int kvx_load_kvcache_q4(int32_t device, int32_t dtype, void* key_dev, void* valu
  * [cu_seqlens_q[0], cu_seqlens_q[num_seqs]) are left as they were. Scores,
  * maxima, sums and outputs are held in fp32; the weights are rounded to the
  * tensor cores' 16-bit type before they meet the values.
+ * A value that is infinite or NaN decides its element of the rows that see it and
+ * reaches no other; a row that shares a tile with it unseen is computed again, at
+ * about 0.4 us a key.
  * A page id outside [0, num_blocks) reads as zeros and is flagged with
  * KVX_DEV_BAD_SRC_ID; a context length outside [0, table_width * block_size] is
  * held in it and a sequence whose cu_seqlens_q entries are out of order or range

@@ -12,6 +12,7 @@
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "kvx.h"
 #include "kvx_device.cuh"
@@ -174,6 +175,7 @@ template <typename T>
 struct Pair;
 template <>
 struct Pair<__nv_bfloat16> {
+    static constexpr int kInf = 0x7f80;
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
         uint32_t r;
         asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -185,6 +187,7 @@ struct Pair<__nv_bfloat16> {
 };
 template <>
 struct Pair<__half> {
+    static constexpr int kInf = 0x7c00;
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
         uint32_t r;
         asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -236,71 +239,179 @@ __device__ __forceinline__ float row_divisor(float amax) {
     return e < 0x0d800000u || e == 0x7f800000u ? 1.f : __uint_as_float(e);
 }
 
-// One element of the cache as fp32 (the rare path below).
+// ---------------------------------------------------------------------------
+// Rows that a masked value spoiled
+// ---------------------------------------------------------------------------
+//
+// A product with a masked key is skipped in the formula, but a tile multiplies every row with every key: weight 0 times
+// a value that is infinite or NaN gives NaN in rows that do not see that key. So does, for an infinity that a row sees, a
+// weight that rounds to 0 or the second part of a weight in two. Such elements (NaN although the row's sum
+// is a number) are computed again from the row's visible keys alone, by a warp a row, when no other warp waits for it. An
+// element that sees values that are not finite has its result from those alone, and a row all of whose elements are NaN by
+// them is left there. Only inputs that are not finite come here.
+
+// A lane's elements of a row of the cache, lane * D / 32 and following, as fp32; zeros for a bad page.
 template <typename T, int D, bool Q4>
-__device__ __forceinline__ float cache_element(const AttnParams& p, const char* plane, int64_t page, int off, int head,
-                                               int d) {
+__device__ __forceinline__ void lane_elements(const AttnParams& p, const char* plane, int64_t page, int off, int head,
+                                              float (&v)[D / 32]) {
+    constexpr int N = D / 32;
+    const int lane = threadIdx.x & 31;
     const char* base = plane + page + head * p.head_stride;
-    if constexpr (Q4) {
-        const uint8_t* b = reinterpret_cast<const uint8_t*>(base);
-        const uint32_t byte = b[off * (D / 2) + d / 2];
-        const uint32_t scale = b[p.block_size * (D / 2) + off * (D / 16) + d / 16];
-        const uint32_t c = d & 1 ? byte >> 4 : byte & 15;
-        const uint32_t e = (c >> 1) & 3;
-        const float level = e ? static_cast<float>((2 + (c & 1)) << e) * 0.25f : 0.5f * (c & 1);
-        return (c & 8 ? -level : level) * Pair<__half>::unpack(scales_to_half(scale)).x;
-    } else {
-        return static_cast<float>(reinterpret_cast<const T*>(base + off * p.slot_stride)[d]);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+        float2 x = make_float2(0.f, 0.f);
+        if (page >= 0) {
+            if constexpr (Q4) {
+                const uint8_t* b = reinterpret_cast<const uint8_t*>(base);
+                // The byte four times over: of a word whose upper bytes are known to be 0, nvcc 12.9 makes zeros.
+                uint32_t h[4];
+                codes_to_half(b[off * (D / 2) + lane * (N / 2) + i] * 0x01010101u, h);
+                const uint32_t scale = b[p.block_size * (D / 2) + off * (D / 16) + lane * N / 16];
+                x = Pair<__half>::unpack(mul_half2(h[0], scales_to_half(scale | (scale << 8))));
+            } else {
+                x = Pair<T>::unpack(reinterpret_cast<const uint32_t*>(base + off * p.slot_stride)[lane * (N / 2) + i]);
+            }
+        }
+        v[2 * i] = x.x;
+        v[2 * i + 1] = x.y;
     }
 }
 
-// A product with a masked key is skipped in the formula, but a tile multiplies
-// every row with every key: weight 0 times a value that is infinite or NaN gives
-// NaN in rows that do not see that key. Such a row (finite sum, NaN in the
-// output) is computed again from its visible keys alone: out[d0 + i], i < N, for
-// the maximum m2 (of scale_log2 * score) that the tiles found. Only inputs that are not finite come here.
-template <typename T, int D, bool Q4, typename F>
-__device__ __forceinline__ void for_visible_keys(const AttnParams& p, const AttnItem& it, const KeyTiles& kt, int tile_keys,
-                                                 int row, F&& each) {
-    const int token = row / p.group;
-    const int head = it.head * p.group + row % p.group;
-    const int pos = it.pos0 + token;
-    const T* q = reinterpret_cast<const T*>(p.q + (it.q0 + token) * p.q_token_stride + head * p.q_head_stride);
-    const int32_t* table = p.table + it.seq * p.table_stride;
-    for (int i = kt.begin; i < kt.end; ++i) {
-        const int first = (i < kt.head ? i : i + kt.skip) * tile_keys;
-        for (int j = first; j < first + tile_keys; ++j) {
-            if (!visible(p, pos, j)) continue;
-            const int blk = j / p.block_size, off = j - blk * p.block_size;
-            const int64_t page = page_offset(p, table, blk);
-            float s = 0.f;
-            if (page >= 0)
-                for (int d = 0; d < D; ++d)
-                    s = fmaf(static_cast<float>(q[d]), cache_element<T, D, Q4>(p, p.k, page, off, it.head, d), s);
-            each(s, page, off);
+// The product of a query row with a row of the cache, by one lane; 0 for a bad page.
+template <typename T, int D, bool Q4>
+__device__ __forceinline__ float row_product(const AttnParams& p, const T* q, int64_t page, int off, int head) {
+    if (page < 0) return 0.f;
+    const char* base = p.k + page + head * p.head_stride;
+    float s = 0.f;
+#pragma unroll 4
+    for (int c = 0; c < D / 8; ++c) {                               // 8 elements at a time
+        const uint4 x = reinterpret_cast<const uint4*>(q)[c];
+        const uint32_t a[4] = {x.x, x.y, x.z, x.w};
+        uint32_t k[4];
+        if constexpr (Q4) {
+            codes_to_half(reinterpret_cast<const uint32_t*>(base + off * (D / 2))[c], k);
+            const uint32_t scale = reinterpret_cast<const uint8_t*>(base)[p.block_size * (D / 2) + off * (D / 16) + c / 2];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) k[i] = mul_half2(k[i], scales_to_half(scale | (scale << 8)));
+        } else {
+            const uint4 y = reinterpret_cast<const uint4*>(base + off * p.slot_stride)[c];
+            k[0] = y.x, k[1] = y.y, k[2] = y.z, k[3] = y.w;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 u = Pair<T>::unpack(a[i]), v = Pair<typename std::conditional<Q4, __half, T>::type>::unpack(k[i]);
+            s = fmaf(u.x, v.x, s);
+            s = fmaf(u.y, v.y, s);
         }
     }
+    return s;
 }
-template <typename T, int D, bool Q4, int N>
-__device__ __noinline__ void visible_keys_only(const AttnParams& p, const AttnItem& it, const KeyTiles& kt, int tile_keys,
-                                               int row, float m2, int d0, float* acc) {
-    for (int i = 0; i < N; ++i) acc[i] = 0.f;
-    for_visible_keys<T, D, Q4>(p, it, kt, tile_keys, row, [&](float s, int64_t page, int off) {
-        if (page < 0) return;                       // reads as zeros
-        const float w = exp2f(fmaf(s, p.scale_log2, -m2));
-        for (int d = 0; d < N; ++d)
-            acc[d] = fmaf(w, cache_element<T, D, Q4>(p, p.v, page, off, it.head, d0 + d), acc[d]);
-    });
+
+// In a 16-bit output, a NaN that is to be computed again (conversions give 0x7fff).
+template <typename T>
+__device__ __forceinline__ constexpr uint16_t marked_nan() {
+    return std::is_same<T, __half>::value ? 0x7e01 : 0x7fc1;
 }
-// Maximum and sum of such a row.
+
+// A warp's work on one finished row: its NaN elements (the marked ones of an output row with `marked`) again. `hint` is a
+// key whose values gave NaN in the row before: the next row mostly has its NaN from there too.
 template <typename T, int D, bool Q4>
-__device__ __noinline__ void visible_scores(const AttnParams& p, const AttnItem& it, const KeyTiles& kt, int tile_keys, int row,
-                                            float* m2, float* sum) {
-    float m = -INFINITY, l = 0.f;
-    for_visible_keys<T, D, Q4>(p, it, kt, tile_keys, row, [&](float s, int64_t, int) { m = fmaxf(m, s * p.scale_log2); });
-    for_visible_keys<T, D, Q4>(p, it, kt, tile_keys, row, [&](float s, int64_t, int) { l += exp2f(fmaf(s, p.scale_log2, -m)); });
-    *m2 = m;
-    *sum = l;
+__device__ __noinline__ void mend_row(const AttnParams& p, const AttnItem& it, const KeyTiles& kt, int tile_keys, int row,
+                                      bool marked, int* hint) {
+    constexpr int N = D / 32;
+    const int lane = threadIdx.x & 31;
+    const int token = row / p.group, head = it.head * p.group + row - token * p.group;
+    const int pos = it.pos0 + token;
+    uint16_t* out = reinterpret_cast<uint16_t*>(p.out + (it.q0 + token) * p.o_token_stride + head * p.o_head_stride) + lane * N;
+    const int64_t at = (static_cast<int64_t>(it.q0 + token) * p.heads + head) * p.splits + it.split;
+    float* part = p.ws_o + at * D + lane * N;
+    uint32_t bad = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const bool nan = p.splits > 1 ? isnan(part[i]) : marked ? out[i] == marked_nan<T>() : (out[i] & 0x7fff) > Pair<T>::kInf;
+        bad |= static_cast<uint32_t>(nan) << i;
+    }
+    if (!__any_sync(~0u, bad)) return;
+
+    // What the element has of values that are not finite: their sum decides it, whatever the weights.
+    float odd[N], acc[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) odd[i] = acc[i] = 0.f;
+    auto covered = [&]() {
+        uint32_t nan = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) nan |= static_cast<uint32_t>(isnan(odd[i])) << i;
+        return __all_sync(~0u, (bad & ~nan) == 0);
+    };
+    const int32_t* table = p.table + it.seq * p.table_stride;
+    bool done = false;
+    if (*hint >= 0 && visible(p, pos, *hint)) {
+        const int blk = block_of(p, *hint);
+        float v[N];
+        lane_elements<T, D, Q4>(p, p.v, page_offset(p, table, blk), *hint - blk * p.block_size, it.head, v);
+#pragma unroll
+        for (int i = 0; i < N; ++i) odd[i] = isnan(v[i]) ? v[i] : 0.f;
+        done = covered();
+        if (!done)
+#pragma unroll
+            for (int i = 0; i < N; ++i) odd[i] = 0.f;
+    }
+    // 32 keys at a time: a lane finds the page and the score of one of them, then their values come row by row.
+    const T* q = reinterpret_cast<const T*>(p.q + (it.q0 + token) * p.q_token_stride + head * p.q_head_stride);
+    float m = -INFINITY, sum = 0.f;                                 // this lane's part of the sum
+    for (int n = kt.begin * (tile_keys / 32); n < kt.end * (tile_keys / 32) && !done; ++n) {
+        const int tile = n / (tile_keys / 32);
+        const int first = (tile < kt.head ? tile : tile + kt.skip) * tile_keys + 32 * (n - tile * (tile_keys / 32));
+        const int j = first + lane;
+        const bool see = visible(p, pos, j);
+        const uint32_t seen = __ballot_sync(~0u, see);
+        if (!seen) continue;
+        const int blk = block_of(p, j), off = j - blk * p.block_size;
+        const int64_t page = see ? page_offset(p, table, blk) : -1;
+        const float s = see ? row_product<T, D, Q4>(p, q, page, off, it.head) * p.scale_log2 : -INFINITY;
+        float next = s;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) next = fmaxf(next, __shfl_xor_sync(~0u, next, d));
+        next = fmaxf(next, m);
+        const float base = next == -INFINITY ? 0.f : next, shrink = exp2f(m - base), w = exp2f(s - base);
+        m = next;
+        sum = fmaf(sum, shrink, w);
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] *= shrink;
+        uint32_t nan = 0;                                           // keys with a NaN among this lane's elements
+#pragma unroll 8
+        for (int u = 0; u < 32; ++u) {
+            float v[N];
+            lane_elements<T, D, Q4>(p, p.v, __shfl_sync(~0u, page, u), __shfl_sync(~0u, off, u), it.head, v);
+            const float weight = __shfl_sync(~0u, w, u);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const bool fine = fabsf(v[i]) < INFINITY;
+                acc[i] = fmaf(weight, fine ? v[i] : 0.f, acc[i]);
+                odd[i] += fine ? 0.f : v[i];
+                nan |= static_cast<uint32_t>(isnan(v[i])) << u;
+            }
+        }
+        done = covered();
+        nan = __reduce_or_sync(~0u, nan);
+        if (done && nan) *hint = first + __ffs(nan) - 1;
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+    // A partial result is in units of the maximum that the row's others are joined with.
+    const float mine = m == -INFINITY ? 0.f : m;
+    float factor = sum > 0.f ? p.out_scale / sum : 0.f;
+    if (p.splits > 1) {
+        const float ref = p.ws_ml[at * 2];
+        factor = exp2f(mine - (ref == -INFINITY ? 0.f : ref));
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float x = odd[i] == 0.f ? acc[i] * factor : odd[i];
+        if (!(bad & (1u << i))) continue;
+        if (p.splits > 1) part[i] = x;
+        else reinterpret_cast<T*>(out)[i] = static_cast<T>(x);
+    }
 }
 
 // ---------------------------------------------------------------------------

@@ -568,6 +568,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, Q4 && NT == 1 ? 4 : 2) attn_
     }
     __syncthreads();
     constexpr int kPairs = D / 2;
+    bool spoiled = false;              // see mend_row
     for (int e = threadIdx.x; e < rows * kPairs; e += kSplitWarps * 32) {
         const int row = e / kPairs, d = 2 * (e - row * kPairs);
         float top = -INFINITY;
@@ -585,8 +586,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, Q4 && NT == 1 ? 4 : 2) attn_
             v[0] = fmaf(f, x.x, v[0]);
             v[1] = fmaf(f, x.y, v[1]);
         }
-        if ((isnan(v[0]) || isnan(v[1])) && !isnan(total) && it.tokens > 1)
-            visible_keys_only<T, D, Q4, 2>(p, it, kt, C::kKeys, row, base, d, v);
+        spoiled |= (isnan(v[0]) || isnan(v[1])) && !isnan(total);
         const int token = it.q0 + row / p.group, head = it.head * p.group + row % p.group;
         if (p.splits == 1) {
             const float inv = total > 0.f ? p.out_scale / total : (total == 0.f ? 0.f : total);
@@ -596,6 +596,14 @@ __global__ void __launch_bounds__(kSplitWarps * 32, Q4 && NT == 1 ? 4 : 2) attn_
             const int64_t at = (static_cast<int64_t>(token) * p.heads + head) * p.splits + it.split;
             *reinterpret_cast<float2*>(p.ws_o + at * D + d) = make_float2(v[0], v[1]);
             if (d == 0) *reinterpret_cast<float2*>(p.ws_ml + at * 2) = make_float2(top, total);
+        }
+    }
+    if (__syncthreads_or(spoiled)) {
+        int hint = -1;
+        for (int row = warp; row < rows; row += kSplitWarps) {
+            bool number = true;
+            for (int w = 0; w < kSplitWarps; ++w) number &= !isnan(sm[(w * kRows + row) * 2 + 1]);
+            if (number) mend_row<T, D, Q4>(p, it, kt, C::kKeys, row, false, &hint);
         }
     }
 }

@@ -318,6 +318,7 @@ struct TileBars {
     uint32_t raw_bad[4];       // 16-key groups of a raw tile that were not copied
     uint32_t tmem;
     uint32_t abort;
+    uint32_t spoiled;          // rows that warps 16-19 are to look over again
 };
 
 // Waits for the barrier's phase; false when another warp gave up or the polls ran out.
@@ -411,22 +412,51 @@ struct ItemWalk {
     }
 };
 
-// Writes a row again from its visible keys alone (see visible_keys_only).
+// Item x of the call (kv heads and splits of a tile of queries follow each other: `per_tile` of them).
+__device__ __forceinline__ void item_of(const AttnParams& p, ItemWalk& walk, int64_t x, int per_tile, TileWork& w) {
+    const int y = static_cast<int>(x / per_tile), rest = static_cast<int>(x - static_cast<int64_t>(y) * per_tile);
+    w.it = walk.tile(p, y);
+    w.it.head = rest / p.splits;
+    w.it.split = rest - w.it.head * p.splits;
+    w.kt = key_tiles<kTileKeys>(p, w.it);
+}
+
+// Marks the NaN elements of an output row whose sum is a number, by the thread that wrote it, and notes in `spoiled` that
+// there are some (there may be where `dst` is null: partial results).
+template <typename T, int D>
+__device__ __noinline__ void mark_row(char* dst, volatile uint32_t* spoiled) {
+    uint16_t* out = reinterpret_cast<uint16_t*>(dst);
+    bool any = dst == nullptr;
+    for (int d = 0; d < D && dst != nullptr; ++d)
+        if ((out[d] & 0x7fff) > Pair<T>::kInf) {
+            out[d] = marked_nan<T>();
+            any = true;
+        }
+    if (any) *spoiled = 1;
+}
+
+// The rows that one of warps 16-19 wrote, looked over once more when the CTA's items are done (see mend_row): nobody
+// waits for this warp then, so that no input can make a wait run out.
 template <typename T, int D, bool Q4>
-__device__ __noinline__ void visible_row(const AttnParams& p, const AttnItem& it, const KeyTiles& kt, int tile_keys, int row,
-                                         char* dst, int64_t at) {
-    float m2, sum = 1.f, v[32];
-    if (p.splits > 1) {
-        m2 = p.ws_ml[at * 2];                       // what the other splits are joined with
-        if (m2 == -INFINITY) m2 = 0.f;
-    } else {
-        visible_scores<T, D, Q4>(p, it, kt, tile_keys, row, &m2, &sum);
-    }
-    for (int c = 0; c < D; c += 32) {
-        visible_keys_only<T, D, Q4, 32>(p, it, kt, tile_keys, row, m2, c, v);
-        for (int k = 0; k < 32; ++k) {
-            if (p.splits > 1) p.ws_o[at * D + c + k] = v[k];
-            else reinterpret_cast<T*>(dst)[c + k] = static_cast<T>(v[k] * (p.out_scale / sum));
+__device__ __noinline__ void mend_items(const AttnParams& p) {
+    ItemWalk walk;
+    const int per_tile = p.kv_heads * p.splits;
+    const int64_t items = walk.start(p) * per_tile;
+    const int base = (threadIdx.x & 127) & ~31;
+    int hint = -1;
+    for (int64_t x = blockIdx.x; x < items; x += gridDim.x) {
+        TileWork w;
+        item_of(p, walk, x, per_tile, w);
+        if (w.kt.begin == w.kt.end) continue;
+        for (int r = 0; r < 64; ++r) {
+            const int row = (r >> 5) * kHalfRows + base + (r & 31), token = row / p.group;
+            if (token >= w.it.tokens) continue;
+            if (p.splits > 1) {
+                const int head = w.it.head * p.group + row - token * p.group;
+                const int64_t at = (static_cast<int64_t>(w.it.q0 + token) * p.heads + head) * p.splits + w.it.split;
+                if (isnan(p.ws_ml[at * 2 + 1])) continue;           // its scores: nothing to mend
+            }
+            mend_row<T, D, Q4>(p, w.it, w.kt, kTileKeys, row, true, &hint);
         }
     }
 }
@@ -578,6 +608,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                 mbar_init(&bars->work_empty[i], kRoles);
             }
             bars->abort = 0;
+            bars->spoiled = 0;
             mbar_init_fence();
         }
     }
@@ -656,13 +687,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                     tc_fence_before();
                     mbar_arrive(&bars->o_free[i]);
                 }
-                if (live && nan && !isnan(sum)) visible_row<T, D, Q4>(p, it, kt, kTileKeys, row, dst, at);
+                if (live && nan && !isnan(sum)) mark_row<T, D>(p.splits > 1 ? nullptr : dst, &bars->spoiled);
             }
             if (n > 0) {
                 phases[0] ^= 1;
                 if (second_tile(p, it)) phases[1] ^= 1;
             }
         }
+        __syncwarp();
+        if (__any_sync(~0u, *reinterpret_cast<volatile uint32_t*>(&bars->spoiled))) mend_items<T, D, Q4>(p);
     } else if (warp >= 12) {
         give_registers<56>();
         if (warp == 12 || warp == 15) {
@@ -779,13 +812,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
             for (int64_t x = blockIdx.x;; x += gridDim.x, ring.next()) {
                 TileWork next = {};
                 next.it.seq = -1;                                    // no more items
-                if (x < items) {
-                    const int y = static_cast<int>(x / per_tile), rest = static_cast<int>(x - static_cast<int64_t>(y) * per_tile);
-                    next.it = walk.tile(p, y);
-                    next.it.head = rest / p.splits;
-                    next.it.split = rest - next.it.head * p.splits;
-                    next.kt = key_tiles<kTileKeys>(p, next.it);
-                }
+                if (x < items) item_of(p, walk, x, per_tile, next);
                 if (!warp_wait(&bars->work_empty[ring.at], ring.phase ^ 1, abort, p.status)) break;
                 if (lane == 0) {
                     bars->work[ring.at] = next;

@@ -578,7 +578,8 @@ def test_random_cases(require_gpu):
 # ----------------------------------------------------------------------------------------------
 
 def attended64(case: Case, window=None, sinks=0) -> ref.Attended:
-    """ref.attention for sizes that a loop over rows is too slow for: the same in 64 bits, a sequence at a time."""
+    """ref.attention for sizes that a loop over rows is too slow for: the same in 64 bits, a sequence at a time. What a
+    row does not see counts nowhere, whatever it is; an infinite or NaN value that it sees decides its element."""
     k_all, v_all = (x.to(DEV) for x in case.values())
     q_all = case.q.to(DEV).double()
     T, Hq, D = q_all.shape
@@ -593,6 +594,8 @@ def attended64(case: Case, window=None, sinks=0) -> ref.Attended:
         j = torch.arange(c)
         blocks, offs = case.tables[s].long()[j // page].to(DEV), (j % page).to(DEV)
         k, v = k_all[blocks, offs].permute(1, 0, 2)[:, None], v_all[blocks, offs].permute(1, 0, 2)[:, None]   # [H, 1, c, D]
+        fine = v.isfinite()
+        v, odd = v.masked_fill(~fine, 0.0), [(v == math.inf).double(), (v == -math.inf).double(), v.isnan().double()]
         step = max(1, (1 << 26) // (Hq * c))
         for a in range(0, n, step):
             b = min(n, a + step)
@@ -605,10 +608,15 @@ def attended64(case: Case, window=None, sinks=0) -> ref.Attended:
                 seen &= (p - at_key < window) | (at_key < sinks)
             score = (q @ k.transpose(-1, -2)) * D ** -0.5
             size = (q.abs() @ k.abs().transpose(-1, -2)) * D ** -0.5
-            reach = max(reach, size.masked_fill(~seen, 0.0).amax().item())
+            reach = max(reach, size.masked_fill(~seen, 0.0).nan_to_num(0.0).amax().item())
             keys = max(keys, int(seen.sum(-1).max()))
-            w = torch.softmax(score.masked_fill(~seen, -math.inf), -1).nan_to_num(0.0)
-            out[rows] = (w @ v).permute(2, 0, 1, 3).flatten(1, 2)
+            w = torch.softmax(score.masked_fill(~seen, -math.inf), -1).masked_fill(~seen.any(-1, keepdim=True), 0.0)
+            o = w @ v
+            if not fine.all():
+                up, down, nan = (seen.double() @ x for x in odd)
+                o = o + torch.where(up > 0, math.inf, 0.0) + torch.where(down > 0, -math.inf, 0.0)
+                o = torch.where(nan > 0, math.nan, o)
+            out[rows] = o.permute(2, 0, 1, 3).flatten(1, 2)
             mass[rows] = (w @ v.abs()).permute(2, 0, 1, 3).flatten(1, 2)
         top = max(top, v.abs().max().item())
     return ref.Attended(out.cpu(), mass.cpu(), reach, keys, top)
@@ -618,8 +626,12 @@ def check64(case: Case, **kw) -> torch.Tensor:
     got = case.call(**kw)
     kt.check_device_status(0)
     want = attended64(case, **kw)
-    err, lim = (got.cpu().double() - want.out).abs(), bound(want, case.dtype, case.q4, case.dim)
-    worst = (err / lim.clamp(min=1e-30)).max().item()
+    fine, res = want.out.isfinite(), got.cpu().double()
+    kind = lambda x: x.masked_fill(fine, 0.0).nan_to_num(7.0, 8.0, 9.0)  # noqa: E731
+    wrong = int((kind(res) != kind(want.out)).sum())
+    assert wrong == 0, f"{wrong} elements that are not finite differ"
+    err, lim = (res - want.out)[fine].abs(), bound(want, case.dtype, case.q4, case.dim)[fine]
+    worst = (err / lim.clamp(min=1e-30)).max().item() if err.numel() else 0.0
     assert not err.isnan().any() and (err <= lim).all(), f"worst error is {worst:.3g} of its bound"
     return got
 
@@ -665,6 +677,70 @@ def test_chunks_whose_keys_are_split(require_gpu, dtype, q4):
         assert -(-sum(q_lens) // 2) * group > 24
         check64(case)
         check64(case, window=2500, sinks=130)
+
+
+def spoil(case: Case, s: int, j: int, what: float, first: int, last: int, plane="v"):
+    """Elements first to last - 1 of key or value j of sequence s, of every kv head, become `what` (in a 4-bit cache
+    their groups of 16 become NaN)."""
+    blk, off = int(case.tables[s, j // case.page]), j % case.page
+    cache = case.k if plane == "k" else case.v
+    if not case.q4:
+        cache[blk, off, :, first:last] = what
+        return
+    H, page, dim = cache.shape[2], case.page, case.dim
+    scales = cache[blk].view(H, -1)[:, page * dim // 2:].view(H, page, dim // 16)
+    scales[:, off, first // 16:-(-last // 16)] = 0x7F
+
+
+# Decode (single tokens, keys split), drafted tokens (the same kernel), chunks (the kernel for many rows, keys split)
+# and prompts (the same, several items a CTA).
+SPOILED = [([3000, 2500], None, 4, 1), ([3000, 2500], [4, 3], 4, 1), ([3000, 2500], [70, 90], 4, 1), ([900, 1400], [900, 700], 32, 8)]
+
+
+@pytest.mark.parametrize("dtype,q4", TYPES, ids=IDS)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("ctx,q_lens,heads,kv_heads", SPOILED, ids=["decode", "draft", "chunk", "prompt"])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (300, 5)])
+def test_values_that_are_not_finite_in_long_contexts(require_gpu, dtype, q4, dim, ctx, q_lens, heads, kv_heads, window, sinks):
+    """Infinities and NaN among the values, some seen by all rows, some by a part of a tile's rows, some of both signs, and
+    a NaN key near the end: each element of each row is what the formula gives, and no wait runs out."""
+    case = Case(ctx, heads, kv_heads, dim, 16, dtype, q4, q_lens=q_lens, seed=19)
+    for s, c in enumerate(ctx):
+        n = 1 if q_lens is None else q_lens[s]
+        for j, what, first, last in ((1, math.inf, 0, 3), (c // 2, math.nan, 17, 18), (c - n // 2 - 1, math.inf, 32, 40),
+                                     (c - n // 3 - 1, -math.inf, 36, 44), (c - 2, math.nan, 50, 51),
+                                     (max(0, c - n - 290), math.nan, 60, 61), (c - n // 4 - 1, -math.inf, 0, 64)):
+            spoil(case, s, j, what, first, last)
+    check64(case, window=window, sinks=sinks)
+    spoil(case, 1, ctx[1] - 2, math.nan, 5, 6, "k")
+    check64(case, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("q4", [False, True])
+def test_a_value_that_is_not_finite_costs_little(require_gpu, q4):
+    """One such value that most rows rightly see takes milliseconds, not seconds (0.16 ms without it, 0.4 to 1.0 with);
+    one at the end, for which 244 rows of four items have to be computed again, 93."""
+    def milliseconds(case):
+        f = at.paged_attention_q4 if q4 else at.paged_attention
+        args = case.q.to(DEV), case.k, case.v, case.tables.to(DEV), case.ctx.to(DEV), 16
+        cu = case.cu.to(DEV)
+        best = math.inf
+        for _ in range(3):
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            start.record()
+            f(*args, cu_seqlens_q=cu)
+            end.record()
+            end.synchronize()
+            best = min(best, start.elapsed_time(end))
+        kt.check_device_status(0)
+        return best
+
+    for ctx, q_lens in (([4096], [4096]), ([20000], [5])):
+        for j, most in ((3, 30), (ctx[0] // 2, 30), (ctx[0] - 3, 500)):      # the last: rows of its own tile do not see it
+            case = Case(ctx, 16, 4, 128, 16, torch.float16, q4, q_lens=q_lens, seed=21)
+            milliseconds(case)
+            spoil(case, 0, j, math.nan, 9, 10)
+            assert milliseconds(case) < most
 
 
 # ----------------------------------------------------------------------------------------------
