@@ -231,6 +231,13 @@ __device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
     return r;
 }
 
+// Weights are 2^(score - maximum + this), a factor that the division by their sum takes out again. As fp16 (a 4-bit cache's
+// products and fp16 ones) a weight is off by 2^-25 at least, however small it is: 131070 keys of 2^-26 of the largest weight,
+// 0.2 % of a row behind a strong sink, were all rounded to 0. Seven binades higher the largest still fits (a maximum may be
+// stale by 2^8: 2^15) and the same weights are exact. bf16 reaches as far down as fp32.
+template <typename M>
+constexpr float kLift = std::is_same<M, __half>::value ? 7.f : 0.f;
+
 // What a row of bf16 queries is divided by on its way to fp16: the power of two below
 // its largest element, which keeps every element within 2^-25 of that one; 1 for
 // rows that are zero, below 2^-100 or not finite.
@@ -403,7 +410,7 @@ __device__ __noinline__ void mend_row(const AttnParams& p, const AttnItem& it, c
     float factor = sum > 0.f ? p.out_scale / sum : 0.f;
     if (p.splits > 1) {
         const float ref = p.ws_ml[at * 2];
-        factor = exp2f(mine - (ref == -INFINITY ? 0.f : ref));
+        factor = exp2f(mine - (ref == -INFINITY ? 0.f : ref) + kLift<typename std::conditional<Q4, __half, T>::type>);
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {

@@ -24,7 +24,7 @@
 // 98 us, 0.53 of the copy rate; one of 131070 keys, 8 rows: 48 us, 0.48 (about 400 instructions of a warp per 16 keys, half of them
 // the widening). A call of a few sequences takes 11 us, of which the launch and the host's call are most.
 // Weights: for a bf16 cache they are split in two bf16 numbers (2^-17 relative;
-// the tensor cores have time to spare here), for fp16 and 4-bit rounded to fp16.
+// the tensor cores have time to spare here), for fp16 and 4-bit rounded to fp16, 2^7 higher (kLift).
 
 #include <atomic>
 #include <climits>
@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, Q4 && NT == 1 ? 4 : 2) attn_
                 top[nt][c] = fmaxf(top[nt][c], __shfl_xor_sync(~0u, top[nt][c], 16));
                 grow |= top[nt][c] > mx[nt][c] + 8.f;              // also from no key to a first one
             }
-        // Rescale only when a row's maximum grows by more than 2^8: until then weights stay below that.
+        // Rescale only when a row's maximum grows by more than 2^8: until then weights stay below that (2^15 with kLift).
         if (__any_sync(~0u, grow)) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, Q4 && NT == 1 ? 4 : 2) attn_
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const float base = mx[nt][c] == -INFINITY ? 0.f : mx[nt][c];
+                const float base = (mx[nt][c] == -INFINITY ? 0.f : mx[nt][c]) - kLift<M>;
 #pragma unroll
                 for (int z = 0; z < NS; ++z) {
                     s[z][nt][c] = exp2_approx(s[z][nt][c] - base);

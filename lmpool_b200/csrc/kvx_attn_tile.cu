@@ -21,7 +21,7 @@
 // u + 1 has its scores already and never waits for a product of its own. (With one
 // buffer of 128 keys it did, for the 1400 clocks of both products: 3300 clocks per 128 keys.)
 // Products of one thread execute in order, so S_i(u + 2) cannot overtake the reading of P_i(u).
-// A row's maximum may be stale by 2^8 (weights stay below 2^8, exact in the sums); only
+// A row's maximum may be stale by 2^8 (weights stay below 2^8, 2^15 in fp16: kLift; exact in the sums); only
 // when it grows by more do the softmax warps rescale O, once O_i += P_i(u - 1) is done.
 //
 // Shared memory holds operand rows of 64 elements (128 bytes) in the 128-byte
@@ -1072,9 +1072,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                 const float old = top;
                 if (grow) top = next;
                 // An infinite score gives NaN, as inf - inf does in the formula.
-                const float ref = top == -INFINITY ? 0.f : top == INFINITY ? NAN : top * scale;
+                const float ref = top == -INFINITY ? 0.f : top == INFINITY ? NAN : top * scale - kLift<M>;
                 if (u > 0 && __any_sync(~0u, grow)) {
-                    const float shrink = !grow ? 1.f : old == -INFINITY ? 0.f : exp2_approx(old * scale - ref);
+                    const float shrink = !grow ? 1.f : old == -INFINITY ? 0.f : exp2_approx(old * scale - kLift<M> - ref);
                     sum *= shrink;
                     if (!(ok = warp_wait(&bars->pv_done[i], pv_phase, abort, p.status))) break;
                     tc_fence_after();

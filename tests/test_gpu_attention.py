@@ -743,6 +743,40 @@ def test_a_value_that_is_not_finite_costs_little(require_gpu, q4):
             assert milliseconds(case) < most
 
 
+@pytest.mark.parametrize("dtype,q4", TYPES, ids=IDS)
+@pytest.mark.parametrize("tokens,copies", [(1, 1200), (3, 1200), (40, 75), (3, 1)], ids=["decode", "draft", "chunk", "split"])
+def test_a_long_tail_behind_strong_sinks_counts(require_gpu, dtype, q4, tokens, copies):
+    """131070 keys, eight strong ones at the start (one for each part of a tile that has a maximum of its own) and a tail of
+    about 2^-26 of their weight each, together 2^-12, whose values alone are not 0. A weight in fp16 is off by at most 2^-25
+    of 2^7 times the largest, so the last term of the bound is n 2^-32 max |v| here. The same sequence many times over
+    leaves the keys of an item in one piece."""
+    n, dim, page, heads = 131070, 64, 256, 2
+    case = Case([n], 4 * heads, heads, dim, page, dtype, q4, q_lens=[tokens], seed=22)
+    g = torch.Generator().manual_seed(23)
+    k, v = torch.zeros(n, heads, dim), 1 + 0.125 * torch.randn(n, heads, dim, generator=g).clamp(-3, 3)
+    k[:, :, 16:32] = 0.25 * torch.randn(n, heads, 16, generator=g)
+    for j in range(0, 128, 16):
+        k[j], v[j] = 0.0, 0.0
+        k[j, :, 0] = 6.0                                            # on the grid of a 4-bit row
+    slots = case.tables[0].long()[torch.arange(n) // page] * page + torch.arange(n) % page
+    (at.store_kvcache_q4 if q4 else at.store_kvcache)(k.to(dtype).to(DEV), v.to(dtype).to(DEV), case.k, case.v, slots.to(DEV), page)
+    case.q = 0.5 * torch.randn(case.q.shape, generator=g)
+    case.q[:, :, 0] = 26 * math.log(2) / 6 * dim ** 0.5
+    case.q = case.q.to(dtype)
+    want = attended64(case)
+    f = at.paged_attention_q4 if q4 else at.paged_attention
+    got = f(case.q.repeat(copies, 1, 1).to(DEV), case.k, case.v, case.tables.repeat(copies, 1).to(DEV),
+            case.ctx.repeat(copies).to(DEV), page,
+            cu_seqlens_q=None if tokens == 1 else torch.arange(copies + 1, dtype=torch.int32, device=DEV) * tokens)
+    kt.check_device_status(0)
+    assert torch.equal(got, got[:tokens].repeat(copies, 1, 1))
+    half = q4 or dtype == torch.float16
+    lim = bound(want, dtype, q4, dim) - want.keys * 2.0 ** -25 * want.top + (want.keys * 2.0 ** -32 * want.top if half else 0.0)
+    assert 2.0 ** -13 < want.out.min() and want.out.max() < 2.0 ** -11 and lim.max() < 2.0 ** -13
+    err = (got[:tokens].cpu().double() - want.out).abs()
+    assert (err <= lim).all(), f"worst error is {(err / lim).max():.3g} of its bound"
+
+
 # ----------------------------------------------------------------------------------------------
 # Refusals
 # ----------------------------------------------------------------------------------------------
