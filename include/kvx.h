@@ -368,7 +368,8 @@ int kvx_load_kvcache_q4(int32_t device, int32_t dtype, void* key_dev, void* valu
  * num_seqs), else cu_seqlens_q[s + 1] - cu_seqlens_q[s]; token rows outside
  * [cu_seqlens_q[0], cu_seqlens_q[num_seqs]) are left as they were. Scores,
  * maxima, sums and outputs are held in fp32; the weights are rounded to the
- * tensor cores' 16-bit type before they meet the values.
+ * tensor cores' 16-bit type before they meet the values. A score beyond fp32's
+ * range is infinite: NaN for its row above, weight 0 below.
  * A value that is infinite or NaN decides its element of the rows that see it and
  * reaches no other; a row that shares a tile with it unseen is computed again, at
  * about 0.4 us a key.

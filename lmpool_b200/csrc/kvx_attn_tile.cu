@@ -70,6 +70,7 @@ constexpr int kHalfRows = 128;                 // rows of one of the two row til
 // on a 4-bit one, where the widening wants the issue slots (prompts on a 4-bit cache: 401 us, 422 with 3).
 template <bool Q4>
 constexpr int kFmaPairs = Q4 ? 1 : 3;
+constexpr float kFarScore = 1 << 20;           // log2 of a weight's factor is off by at most 2^-4 below this
 constexpr uint32_t kMaxWaitPolls = 1u << 22;   // each poll may suspend for a hardware-chosen time
 
 template <int D, bool Q4>
@@ -1071,20 +1072,37 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                 const bool grow = u == 0 || (!(next == top) && !((next - top) * scale <= 8.f));
                 const float old = top;
                 if (grow) top = next;
-                // An infinite score gives NaN, as inf - inf does in the formula.
-                const float ref = top == -INFINITY ? 0.f : top == INFINITY ? NAN : top * scale - kLift<M>;
-                if (u > 0 && __any_sync(~0u, grow)) {
-                    const float shrink = !grow ? 1.f : old == -INFINITY ? 0.f : exp2_approx(old * scale - kLift<M> - ref);
-                    sum *= shrink;
-                    if (!(ok = warp_wait(&bars->pv_done[i], pv_phase, abort, p.status))) break;
-                    tc_fence_after();
+                // A score that is infinite, itself or only when scaled, gives NaN, as inf - inf does in the formula.
+                const float lead = top * scale;
+                float ref = lead == -INFINITY ? 0.f : lead == INFINITY ? NAN : lead - kLift<M>;
+                // Below, score * scale - ref is rounded once, so that the largest weight is off by 2 to the rounding of `lead`:
+                // a factor that the sum has too, but one that must stay small. Rows of larger scores subtract first. (One
+                // vote for both rare cases: with two, prompts take 2 % longer.)
+                const bool far = fabsf(lead) >= kFarScore && lead != -INFINITY;
+                if (__any_sync(~0u, grow || far)) {
+                    if (u > 0 && __any_sync(~0u, grow)) {
+                        const float shrink = !grow ? 1.f : old == -INFINITY ? 0.f : exp2_approx((old - top) * scale);
+                        sum *= shrink;
+                        if (!(ok = warp_wait(&bars->pv_done[i], pv_phase, abort, p.status))) break;
+                        tc_fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < D; c += 8) {
-                        uint32_t o[8];
-                        tmem_load8(o_at + c, o);
+                        for (int c = 0; c < D; c += 8) {
+                            uint32_t o[8];
+                            tmem_load8(o_at + c, o);
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * shrink);
-                        tmem_store8(o_at + c, o);
+                            for (int k = 0; k < 8; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * shrink);
+                            tmem_store8(o_at + c, o);
+                        }
+                    }
+                    if (__any_sync(~0u, far)) {
+                        const float zero = top == -INFINITY ? 0.f : top;
+                        ref = ref == ref ? -kLift<M> : ref;
+#pragma unroll
+                        for (int c = 0; c < kStepKeys; c += 2) {
+                            const float2 d = unpair(add2(pair2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), pair2(-zero, -zero)));
+                            sr[c] = __float_as_uint(d.x);
+                            sr[c + 1] = __float_as_uint(d.y);
+                        }
                     }
                 }
                 const uint64_t scale2 = pair2(scale, scale), ref2 = pair2(-ref, -ref);

@@ -777,6 +777,54 @@ def test_a_long_tail_behind_strong_sinks_counts(require_gpu, dtype, q4, tokens, 
     assert (err <= lim).all(), f"worst error is {(err / lim).max():.3g} of its bound"
 
 
+@pytest.mark.parametrize("q_lens", [None, [3, 2], [40, 30]], ids=["decode", "draft", "chunk"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_scores_beyond_fp32_are_infinite(require_gpu, dim, q_lens):
+    """Products that fit into fp32 until they are scaled: NaN for the rows that see one, the others as ever."""
+    case = Case([90, 70], 4, 1, dim, 16, torch.bfloat16, False, q_lens=q_lens, seed=24)
+    case.q[:, 0] *= 2.0 ** 50                                       # one head of four
+    case.k *= 2.0 ** 65
+    got = case.call(scale=2.0 ** 14)
+    kt.check_device_status(0)
+    assert got[:, 0].isnan().all() and got[:, 1:].isfinite().all() and got[:, 1:].abs().amax(-1).gt(0).all()
+
+
+@pytest.mark.parametrize("dtype,q4", TYPES, ids=IDS)
+@pytest.mark.parametrize("ctx,q_lens", [([300, 200], None), ([300, 200], [3, 2]), ([300, 200], [40, 30]), ([4000], [60])],
+                         ids=["decode", "draft", "chunk", "split"])
+def test_scores_far_apart_leave_the_key_of_the_largest(require_gpu, dtype, q4, ctx, q_lens):
+    """Scores of 2^26 and more: their roundings are far larger than 1, and what is left of a row is the value of its best key."""
+    dim = 64
+    case = Case(ctx, 4, 1, dim, 16, dtype, q4, q_lens=q_lens, seed=25)
+    size = 2.0 ** 13 if dtype == torch.float16 else 2.0 ** 25
+    case.q = (case.q.float().clamp(-4, 4) * size).to(dtype)
+    if not q4:
+        case.k = (case.k.float().clamp(-4, 4) * 2.0 ** 13).to(dtype)
+    k, v = case.values()
+    got = case.call().cpu().double()
+    kt.check_device_status(0)
+    cu = case.cu.tolist() if case.cu is not None else range(len(ctx) + 1)
+    clear = 0
+    for s, c in enumerate(ctx):
+        j = torch.arange(c)
+        ids = case.tables[s].long()[j // 16]
+        keys, values = k[ids, j % 16, 0], v[ids, j % 16, 0]
+        for t in range(cu[s], cu[s + 1]):
+            p = c - cu[s + 1] + t
+            q = case.q[t].double()
+            score, reach = q @ keys[:p + 1].T * dim ** -0.5, (q.abs() @ keys[:p + 1].abs().T * dim ** -0.5).amax()
+            (first, second), best = score.topk(2, -1).values.unbind(-1), score.argmax(-1)
+            # each score is off by (D + 8) half steps of fp32 at most; other keys' weights stay below 2^-40
+            sure = first - second > 2 * (dim + 8) * 2.0 ** -24 * reach + 40
+            clear += int(sure.sum())
+            err = (got[t] - values[best]).abs()
+            # half a step of the output, and half a step of the best key's weight, which is rounded for the products (it is
+            # 2^x, x the rounding of score * scale) but not in their sum: w (1 + d) v / w
+            step = HALF_STEP[dtype] + (2.0 ** -11 if q4 else HALF_STEP[dtype])
+            assert (err <= step * (1 + 2.0 ** -8) * values[best].abs() + 2.0 ** -30 * values.abs().max())[sure].all()
+    assert clear > (4 if q_lens is None else 2 * sum(q_lens))
+
+
 # ----------------------------------------------------------------------------------------------
 # Refusals
 # ----------------------------------------------------------------------------------------------
