@@ -103,8 +103,8 @@ __global__ void __launch_bounds__(kQ4Threads) store_q4_kernel(const __grid_const
 #pragma unroll
     for (int i = 0; i < 8; ++i) most = max_u16x2(most, raw[i] & 0x7fff7fffu);
     most = max(most & 0xffffu, most >> 16);
-    const float amax = Pair<T>::unpack(most).x * mul;
-    const bool finite = amax < INFINITY;
+    const bool finite = most < Pair<T>::kInf;
+    const float amax = Pair<T>::unpack(most).x * mul;               // may overflow: the scale saturates
     uint16_t scale2;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %1;" : "=h"(scale2) : "f"(__fdiv_rn(amax, 6.f)));
     const float s = Pair<__half>::unpack(scales_to_half(scale2)).x;

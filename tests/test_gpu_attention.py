@@ -165,6 +165,27 @@ def test_q4_scales_shift_the_range(require_gpu):
             assert torch.equal(v[t, h].cpu().double(), want * 2.0 ** 16)
 
 
+def test_q4_rows_beyond_fp32_saturate(require_gpu):
+    """Finite elements that k_scale or v_scale below 1 lifts out of fp32's range are held at the largest value, as any that
+    are too large; groups with an infinity or a NaN still read back as NaN."""
+    T, H, D, page = 4, 1, 64, 16
+    x = torch.randn(T, H, D, generator=torch.Generator().manual_seed(26)).to(torch.bfloat16)
+    x[0] *= 2.0 ** 125
+    x[1, 0, 5] = -2.0 ** 127
+    x[2, 0, 20] = torch.finfo(torch.bfloat16).max
+    x[2, 0, 50] = math.inf
+    x[3, 0, 3] = math.nan
+    kc = torch.zeros(1, page, H, at.q4_row_bytes(D), dtype=torch.uint8, device=DEV)
+    vc = torch.zeros_like(kc)
+    at.store_kvcache_q4(x.to(DEV), x.to(DEV), kc, vc, torch.arange(T, device=DEV), page, k_scale=0.5, v_scale=2.0 ** -64)
+    kt.check_device_status(0)
+    for cache, scale in ((kc, 0.5), (vc, 2.0 ** -64)):
+        want = torch.zeros(1, page, H, at.q4_row_bytes(D), dtype=torch.uint8)
+        for t in range(T):
+            ref.q4_write(want, t, 0, *ref.q4_encode_row(x[t, 0].double() / scale))
+        assert torch.equal(cache.cpu(), want)
+
+
 def test_q4_strided_rows_and_views_of_a_stacked_cache(require_gpu):
     """Rows cut out of a fused projection, a cache that is one layer of [2, L, N, ...], and a slot list with gaps."""
     T, H, D, page, L, N = 21, 2, 64, 16, 3, 4
