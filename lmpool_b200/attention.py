@@ -201,12 +201,18 @@ def _same_device(first: torch.Tensor, *others: torch.Tensor) -> int:
 
 
 def _rows_of(x: torch.Tensor) -> torch.Tensor:
-    """16-bit x [T, H, D] with contiguous, 16-byte aligned token rows (a copy where it has none)."""
-    _, H, D = x.shape
+    """16-bit x [T, H, D] with contiguous, 16-byte aligned token rows (a copy where it has none). The stride of a
+    dimension of one entry is not used and may be anything."""
+    T, H, D = x.shape
     st = x.stride()
-    if st[2] == 1 and (H == 1 or st[1] == D) and st[0] % 8 == 0 and x.data_ptr() % 16 == 0:
+    if st[2] == 1 and (H == 1 or st[1] == D) and (T == 1 or st[0] % 8 == 0) and x.data_ptr() % 16 == 0:
         return x
-    return x.contiguous() if not x.is_contiguous() else x.clone()
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+def _token_stride(x: torch.Tensor) -> int:
+    """Bytes from a token's row of 16-bit x [T, H, D] to the next one's; a single token's is that of its row."""
+    return 2 * x.stride(0) if x.shape[0] > 1 else 2 * x.shape[1] * x.shape[2]
 
 
 def _check_slots(slot_mapping: torch.Tensor) -> torch.Tensor:
@@ -250,7 +256,7 @@ def store_kvcache_q4(
         return
     key, value = _rows_of(key), _rows_of(value)
     rc = _capi.lib().kvx_store_kvcache_q4(
-        device, _DTYPE_CODE[key.dtype], key.data_ptr(), value.data_ptr(), key.stride(0) * 2, value.stride(0) * 2,
+        device, _DTYPE_CODE[key.dtype], key.data_ptr(), value.data_ptr(), _token_stride(key), _token_stride(value),
         k_cache.data_ptr(), v_cache.data_ptr(), block_stride, slot_mapping.data_ptr(), T, num_blocks, block_size, H, D,
         k_scale, v_scale, _status(device), _raw_stream(device))
     if rc:
@@ -370,21 +376,24 @@ def _paged_attention(query, k_cache, v_cache, block_tables, context_lens, block_
         raise ValueError(f"window must be positive (None: every key), got {window}")
     if sinks < 0:
         raise ValueError(f"sinks must not be negative, got {sinks}")
+    # The stride of a dimension of one entry is not used and may be anything.
     qs = query.stride()
-    if qs[2] != 1 or qs[0] % 8 or qs[1] % 8 or query.data_ptr() % 16:
-        query = query.contiguous() if not query.is_contiguous() else query.clone()
-        qs = query.stride()
+    q_step, q_head = qs[0] if T > 1 else heads * D, qs[1] if heads > 1 else D
+    if qs[2] != 1 or q_step % 8 or q_head % 8 or query.data_ptr() % 16:
+        query = query.clone(memory_format=torch.contiguous_format)
+        q_step, q_head = heads * D, D
     if out is None:
         out = torch.empty_like(query, memory_format=torch.contiguous_format)
-        os = (heads * D, D)
+        o_step, o_head = heads * D, D
     else:
         if out.shape != query.shape or out.dtype != dtype:
             raise RuntimeError("out must have query's shape and dtype")
         _same_device(query, out)
         os = out.stride()
-        if os[2] != 1 or os[0] % 8 or os[1] % 8 or out.data_ptr() % 16:
+        o_step, o_head = os[0] if T > 1 else heads * D, os[1] if heads > 1 else D
+        if os[2] != 1 or o_step % 8 or o_head % 8 or out.data_ptr() % 16:
             raise RuntimeError("out must have contiguous, 16-byte aligned rows of head_dim")
-        if (heads > 1 and os[1] < D) or (T > 1 and os[0] < D):
+        if (heads > 1 and o_head < D) or (T > 1 and o_step < D):
             raise RuntimeError("out's rows must not overlap")
         if out.data_ptr() == query.data_ptr() and T:
             raise RuntimeError("out must not be the query")
@@ -401,8 +410,8 @@ def _paged_attention(query, k_cache, v_cache, block_tables, context_lens, block_
     rc = _capi.lib().kvx_paged_attention(
         device,
         _capi.pack_attention(query.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-                             block_tables.data_ptr(), context_lens.data_ptr(), cu, 2 * qs[0], 2 * qs[1], 2 * os[0],
-                             2 * os[1], block_stride, slot_stride, head_stride, table_stride, num_blocks, *sizes),
+                             block_tables.data_ptr(), context_lens.data_ptr(), cu, 2 * q_step, 2 * q_head, 2 * o_step,
+                             2 * o_head, block_stride, slot_stride, head_stride, table_stride, num_blocks, *sizes),
         workspace, need, _status(device), _raw_stream(device))
     if rc:
         _capi.check(rc, "kvx_paged_attention")

@@ -140,3 +140,16 @@ def test_cpu_tensors_are_refused():
     kv = torch.zeros(1, 16, 1, 64, dtype=torch.float16)
     with pytest.raises(RuntimeError, match="CUDA"):
         at.paged_attention(x, kv, kv, torch.zeros(2, 1, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), 16)
+
+
+@pytest.mark.parametrize("shape,strides,offset,copied", [
+    ((1, 4, 64), (257, 64, 1), 0, False), ((1, 4, 64), (3, 64, 1), 0, False), ((3, 1, 64), (64, 5, 1), 0, False),
+    ((1, 1, 64), (7, 9, 1), 0, False), ((1, 4, 64), (257, 64, 1), 1, True), ((1, 4, 64), (257, 72, 1), 0, True),
+    ((3, 4, 64), (257, 64, 1), 0, True), ((3, 4, 64), (264, 64, 1), 0, False), ((1, 4, 64), (1, 1, 4), 0, True)])
+def test_rows_to_store_have_strides_that_the_library_takes(shape, strides, offset, copied):
+    x = torch.arange(2048).to(torch.bfloat16).as_strided(shape, strides, offset)
+    rows = at._rows_of(x)
+    assert torch.equal(rows, x) and (rows.data_ptr() != x.data_ptr()) == copied
+    assert rows.data_ptr() % 16 == 0 and at._token_stride(rows) % 16 == 0
+    assert rows.stride(2) == 1 and (shape[1] == 1 or rows.stride(1) == shape[2])
+    assert shape[0] == 1 or at._token_stride(rows) == 2 * rows.stride(0)

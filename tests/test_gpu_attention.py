@@ -846,6 +846,32 @@ def test_scores_far_apart_leave_the_key_of_the_largest(require_gpu, dtype, q4, c
     assert clear > (4 if q_lens is None else 2 * sum(q_lens))
 
 
+@pytest.mark.parametrize("q4", [False, True])
+def test_a_single_token_or_head_may_have_any_stride(require_gpu, q4):
+    """The stride of a dimension of one entry of the query, of `out` and of the rows to store means nothing."""
+    f = at.paged_attention_q4 if q4 else at.paged_attention
+    for heads, tokens in ((4, 1), (1, 1), (1, 3)):
+        case = Case([70], heads, 1, 64, 16, torch.bfloat16, q4, q_lens=[tokens], seed=27)
+        want = case.check()
+        strides = (257 if tokens == 1 else heads * 64, 3 if heads == 1 else 64, 1)
+        memory = torch.zeros(2, 2048, dtype=torch.bfloat16, device=DEV)
+        q, out = (m.as_strided(case.q.shape, strides) for m in memory)
+        q.copy_(case.q)
+        got = f(q, case.k, case.v, case.tables.to(DEV), case.ctx.to(DEV), 16, cu_seqlens_q=case.cu.to(DEV), out=out)
+        assert got.data_ptr() == out.data_ptr() and torch.equal(got, want)
+        odd = torch.zeros(2049, dtype=torch.bfloat16, device=DEV)[1:].as_strided(case.q.shape, strides)
+        odd.copy_(case.q)
+        assert torch.equal(f(odd, case.k, case.v, case.tables.to(DEV), case.ctx.to(DEV), 16, cu_seqlens_q=case.cu.to(DEV)), want)
+    x = torch.randn(1, 2, 64, generator=torch.Generator().manual_seed(28)).to(torch.bfloat16)
+    caches = [torch.zeros(1, 16, 2, at.q4_row_bytes(64), dtype=torch.uint8, device=DEV) for _ in range(4)]
+    slot = torch.tensor([3], device=DEV)
+    at.store_kvcache_q4(x.to(DEV), x.to(DEV), caches[0], caches[1], slot, 16)
+    odd = torch.zeros(2, 512, dtype=torch.bfloat16, device=DEV).as_strided((2, 1, 2, 64), (512, 131, 64, 1))
+    odd.copy_(x.expand(2, 1, 2, 64))
+    at.store_kvcache_q4(odd[0], odd[1], caches[2], caches[3], slot, 16)
+    assert int(caches[0].sum()) > 0 and torch.equal(caches[0], caches[2]) and torch.equal(caches[1], caches[3])
+
+
 # ----------------------------------------------------------------------------------------------
 # Refusals
 # ----------------------------------------------------------------------------------------------
