@@ -301,6 +301,26 @@ def load_kvcache_q4(
 # Attention over the paged cache
 # ---------------------------------------------------------------------------
 
+def _rows_overlap(tokens: int, token_stride: int, heads: int, head_stride: int, size: int) -> bool:
+    """Whether two of the rows of ``size`` elements at ``t * token_stride + h * head_stride`` share one."""
+    if tokens == 0 or heads == 0:
+        return False
+    if tokens == 1 or heads == 1:
+        return tokens * heads > 1 and (token_stride if tokens > 1 else head_stride) < size
+    (small, n), (large, m) = sorted(((token_stride, tokens), (head_stride, heads)))
+    if small < size:
+        return True
+    span = (n - 1) * small + size
+    if large >= span:
+        return False
+    # Crossed: a step along the large stride ends between two rows of the small one.
+    for far in range(large, min(m * large, span), large):
+        rest = far % small
+        if rest < size or (small - rest < size and far + small - rest < span):
+            return True
+    return False
+
+
 @functools.lru_cache(maxsize=1024)
 def _attention_workspace(device: int, ragged: bool, sizes: tuple) -> int:
     """Bytes of scratch that a call needs: its sizes alone decide."""
@@ -393,7 +413,7 @@ def _paged_attention(query, k_cache, v_cache, block_tables, context_lens, block_
         o_step, o_head = os[0] if T > 1 else heads * D, os[1] if heads > 1 else D
         if os[2] != 1 or o_step % 8 or o_head % 8 or out.data_ptr() % 16:
             raise RuntimeError("out must have contiguous, 16-byte aligned rows of head_dim")
-        if (heads > 1 and o_head < D) or (T > 1 and o_step < D):
+        if _rows_overlap(T, o_step, heads, o_head, D):
             raise RuntimeError("out's rows must not overlap")
         if out.data_ptr() == query.data_ptr() and T:
             raise RuntimeError("out must not be the query")

@@ -1,6 +1,7 @@
 """CPU tests of the 4-bit cache's definition and of the refusals that need no GPU."""
 import ctypes
 import math
+import random
 import shutil
 import struct
 import subprocess
@@ -153,3 +154,17 @@ def test_rows_to_store_have_strides_that_the_library_takes(shape, strides, offse
     assert rows.data_ptr() % 16 == 0 and at._token_stride(rows) % 16 == 0
     assert rows.stride(2) == 1 and (shape[1] == 1 or rows.stride(1) == shape[2])
     assert shape[0] == 1 or at._token_stride(rows) == 2 * rows.stride(0)
+
+
+def test_rows_that_share_elements_are_found():
+    """Against all pairs, over layouts of every kind: nested, crossed, repeated."""
+    rng = random.Random(1)
+    seen = [0, 0]
+    for _ in range(4000):
+        size, tokens, heads = rng.choice((4, 8)), rng.randint(0, 5), rng.randint(0, 5)
+        step, head = (rng.choice((0, size // 2, size, rng.randint(0, 6) * size, rng.randint(0, 50))) for _ in range(2))
+        starts = sorted(t * step + h * head for t in range(tokens) for h in range(heads))
+        want = any(b - a < size for a, b in zip(starts, starts[1:]))
+        assert at._rows_overlap(tokens, step, heads, head, size) == want, (tokens, step, heads, head, size)
+        seen[want] += 1
+    assert min(seen) > 500

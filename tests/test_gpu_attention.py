@@ -964,3 +964,17 @@ def test_an_output_whose_rows_share_memory_is_refused(require_gpu):
                 torch.empty(2, 1, 64, dtype=torch.bfloat16, device=DEV).expand(2, 4, 64)):
         with pytest.raises(RuntimeError, match="must not overlap"):
             at.paged_attention(q, cache, cache.clone(), tables, ctx, 16, out=out)
+
+
+def test_an_output_whose_tokens_and_heads_share_rows_is_refused(require_gpu):
+    q = torch.zeros(2, 4, 64, dtype=torch.bfloat16, device=DEV)
+    cache = torch.zeros(2, 16, 2, 64, dtype=torch.bfloat16, device=DEV)
+    tables = torch.zeros(2, 1, dtype=torch.int32, device=DEV)
+    ctx = torch.ones(2, dtype=torch.int32, device=DEV)
+    memory = torch.empty(4096, dtype=torch.bfloat16, device=DEV)
+    for strides in ((64, 64, 1), (128, 64, 1), (64, 96, 1), (128, 128, 1)):
+        with pytest.raises(RuntimeError, match="must not overlap"):
+            at.paged_attention(q, cache, cache.clone(), tables, ctx, 16, out=memory.as_strided(q.shape, strides))
+    for strides in ((64, 128, 1), (256, 64, 1), (192, 128, 1)):
+        got = at.paged_attention(q, cache, cache.clone(), tables, ctx, 16, out=memory.as_strided(q.shape, strides))
+        assert got.eq(0).all()
