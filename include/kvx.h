@@ -375,8 +375,8 @@ int kvx_load_kvcache_q4(int32_t device, int32_t dtype, void* key_dev, void* valu
  * about 0.4 us a key.
  * A page id outside [0, num_blocks) reads as zeros and is flagged with
  * KVX_DEV_BAD_SRC_ID; a context length outside [0, table_width * block_size] is
- * held in it and a sequence whose cu_seqlens_q entries are out of order or range
- * is skipped (its rows are undefined), both flagged with KVX_DEV_BAD_LEN.
+ * held in it, and where cu_seqlens_q entries are out of order or range the rows of
+ * the call are undefined, both flagged with KVX_DEV_BAD_LEN.
  * All device reads of lengths, tables and data follow earlier work on `stream`;
  * nothing is read on the host, so the call can be captured and replayed with
  * other lengths. `workspace_dev` holds partial results where the keys are split

@@ -69,6 +69,12 @@ __device__ __forceinline__ int context_of(const AttnParams& p, int s) {
     return static_cast<int>(c);
 }
 
+// Flags cu_seqlens_q entries of sequence s that are out of order or range. The search below may pass over one.
+__device__ __forceinline__ void check_offsets(const AttnParams& p, int s) {
+    const int a = p.cu[s], b = p.cu[s + 1];
+    if (a < 0 || b < a || b > p.num_tokens) atomicOr(p.status, KVX_DEV_BAD_LEN);
+}
+
 // Tile slot `x` of a call. Without cu_seqlens a slot is a sequence. With them
 // the slots of sequence s start at cu[s] / tile + s: that leaves every
 // sequence at least ceil(len / tile) of them, needs no prefix sum and no

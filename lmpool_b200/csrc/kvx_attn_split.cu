@@ -130,6 +130,9 @@ __global__ void __launch_bounds__(kSplitWarps * 32, Q4 && NT == 1 ? 4 : 2) attn_
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
+    // Every sequence is looked at by one thread of the call (there are at least num_seqs slots).
+    if (p.cu != nullptr && threadIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && blockIdx.x < p.num_seqs)
+        check_offsets(p, blockIdx.x);
     AttnItem it = locate_item(p, blockIdx.x);
     it.head = blockIdx.y;
     it.split = blockIdx.z;

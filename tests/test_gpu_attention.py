@@ -978,3 +978,20 @@ def test_an_output_whose_tokens_and_heads_share_rows_is_refused(require_gpu):
     for strides in ((64, 128, 1), (256, 64, 1), (192, 128, 1)):
         got = at.paged_attention(q, cache, cache.clone(), tables, ctx, 16, out=memory.as_strided(q.shape, strides))
         assert got.eq(0).all()
+
+
+@pytest.mark.parametrize("q4", [False, True])
+@pytest.mark.parametrize("heads", [1, 20])
+def test_offsets_out_of_order_are_flagged_wherever_they_stand(require_gpu, q4, heads):
+    """Also where the search for a sequence passes over the one whose end is before its start (heads: either kernel)."""
+    good = [0, 1, 2, 4, 6, 8, 12, 16]
+    case = Case([20] * 7, heads, 1, 64, 16, torch.float16, q4, q_lens=[b - a for a, b in zip(good, good[1:])], seed=29)
+    case.call()
+    kt.check_device_status(0)
+    for i, bad in ((2, 9), (1, 13), (6, 3), (3, 17), (5, -1), (7, 11), (0, 2)):
+        cu = list(good)
+        cu[i] = bad
+        case.cu = torch.tensor(cu, dtype=torch.int32)
+        case.call()
+        with pytest.raises(_capi.KvxError, match="length"):
+            kt.check_device_status(0)
