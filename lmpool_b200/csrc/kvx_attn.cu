@@ -43,6 +43,8 @@ static int check_args(const kvx_attention* a) {
     if (a->cache_bits != 16 && a->cache_bits != 4) return fail(KVX_EINVAL, "cache_bits must be 16 or 4");
     if (a->head_dim != 64 && a->head_dim != 128) return fail(KVX_EINVAL, "head_dim must be 64 or 128 (got %d)", a->head_dim);
     if (a->num_tokens < 0 || a->num_seqs < 0) return fail(KVX_EINVAL, "negative token or sequence count");
+    if (static_cast<int64_t>(a->num_tokens) + a->num_seqs > INT_MAX)     // slots of items are counted in 32 bits
+        return fail(KVX_EINVAL, "num_tokens + num_seqs is beyond 2^31 - 1");
     if (a->num_heads <= 0 || a->num_kv_heads <= 0 || a->num_heads % a->num_kv_heads != 0)
         return fail(KVX_EINVAL, "num_heads (%d) must be a multiple of num_kv_heads (%d)", a->num_heads, a->num_kv_heads);
     if (a->num_kv_heads > 65535) return fail(KVX_EINVAL, "num_kv_heads must be at most 65535");

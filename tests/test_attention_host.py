@@ -84,6 +84,13 @@ def test_4bit_pages_beyond_32_bit_offsets_are_refused(kvx_lib, dim, bs):
         assert rc == _capi.KVX_EINVAL and b"too large" in kvx_lib.kvx_last_error()
 
 
+def test_more_tokens_and_sequences_than_items_are_counted_for_are_refused(kvx_lib):
+    need = ctypes.c_uint64(0)
+    for sizes in (dict(T=2 ** 31 - 1, S=1), dict(T=2 ** 30, S=2 ** 30), dict(T=2, S=2 ** 31 - 1)):
+        rc = kvx_lib.kvx_attention_workspace(0, _args(cu=1 << 20, **sizes), ctypes.byref(need))
+        assert rc == _capi.KVX_EINVAL and b"beyond" in kvx_lib.kvx_last_error()
+
+
 def test_the_packed_struct_is_the_headers(kvx_lib, tmp_path):
     """pack_attention writes kvx_attention field by field: same size, same places."""
     src = tmp_path / "layout.c"
