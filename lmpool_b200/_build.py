@@ -11,9 +11,12 @@ from __future__ import annotations
 
 import argparse
 import os
+import re
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -28,15 +31,16 @@ NVCC_FLAGS = [
     "-O3",
     "-std=c++17",
     "-lineinfo",
-    "-shared",
     "-Xcompiler",
     "-fPIC,-O2",
-    "-cudart",
-    "static",
     "--expt-relaxed-constexpr",
-    "--threads",
-    "0",
+    "-Xptxas",
+    "-v",
 ]
+LINK_FLAGS = ["-shared", "-Xcompiler", "-fPIC,-O2", "-cudart", "static"]
+# Registers a thread of the kernels whose warps pass registers on to each other (setmaxnreg): their shares add up to
+# what the block was launched with, so a build with any other number must not leave here.
+REGISTERS = {"attn_tile_kernel": 96}
 
 
 def nvcc_path() -> str:
@@ -53,22 +57,48 @@ def is_stale() -> bool:
     return any(p.stat().st_mtime > out_m for p in SOURCES + HEADERS)
 
 
+def check_registers(ptxas_output: str) -> None:
+    """Raises unless every kernel named in REGISTERS was built, with that many registers a thread."""
+    found = {name: [] for name in REGISTERS}
+    kernel = None
+    for line in ptxas_output.splitlines():
+        entry = re.search(r"Compiling entry function '(\w+)'", line)
+        if entry:
+            kernel = next((name for name in REGISTERS if name in entry.group(1)), None)
+        used = re.search(r"Used (\d+) registers", line)
+        if used and kernel:
+            found[kernel].append(int(used.group(1)))
+            kernel = None
+    for name, counts in found.items():
+        if not counts or any(n != REGISTERS[name] for n in counts):
+            raise RuntimeError(f"{name} must be built with {REGISTERS[name]} registers a thread, this nvcc gave {counts}: "
+                               f"its shares of setmaxnreg have to be set anew")
+
+
 def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> Path:
     """Compile the library if a source is newer than the built file."""
     if not force and not is_stale():
         return OUTPUT
     tmp = OUTPUT.with_suffix(".so.tmp")
-    cmd = [nvcc_path(), *ARCH_FLAGS, *NVCC_FLAGS, "-I", str(REPO_ROOT / "include"), "-I", str(PKG_DIR / "csrc")]
+
+    def run(*args: str) -> str:
+        cmd = [nvcc_path(), *ARCH_FLAGS, *args]
+        if verbose:
+            print(" ".join(cmd), file=sys.stderr)
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+        return res.stdout + res.stderr
+
+    # A process per source, so that what ptxas says of one does not mix with another's.
+    with tempfile.TemporaryDirectory() as folder, ThreadPoolExecutor() as pool:
+        objects = [str(Path(folder) / f"{src.stem}.o") for src in SOURCES]
+        include = ["-I", str(REPO_ROOT / "include"), "-I", str(PKG_DIR / "csrc")]
+        output = "".join(pool.map(lambda src, obj: run(*NVCC_FLAGS, *include, "-c", "-o", obj, str(src)), SOURCES, objects))
+        check_registers(output)
+        output += run(*LINK_FLAGS, "-o", str(tmp), *objects)
     if ptxas_info:
-        cmd += ["-Xptxas", "-v"]
-    cmd += ["-o", str(tmp), *map(str, SOURCES)]
-    if verbose:
-        print(" ".join(cmd), file=sys.stderr)
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
-    if verbose or ptxas_info:
-        sys.stderr.write(res.stdout + res.stderr)
+        sys.stderr.write(output)
     os.replace(tmp, OUTPUT)
     return OUTPUT
 

@@ -10,7 +10,7 @@ from pathlib import Path
 import pytest
 import torch
 
-from lmpool_b200 import _capi
+from lmpool_b200 import _build, _capi
 from lmpool_b200 import attention as at
 from oracle import attention_ref as ref
 
@@ -175,3 +175,17 @@ def test_rows_that_share_elements_are_found():
         assert at._rows_overlap(tokens, step, heads, head, size) == want, (tokens, step, heads, head, size)
         seen[want] += 1
     assert min(seen) > 500
+
+
+def _ptxas(*kernels):
+    return "\n".join(f"ptxas info    : Compiling entry function '{name}' for 'sm_100a'\nptxas info    : Function properties for "
+                     f"{name}\n    0 bytes stack frame\nptxas info    : Used {n} registers, used 1 barriers" for name, n in kernels)
+
+
+def test_a_build_with_other_register_counts_is_refused():
+    """The tile kernel's warps pass registers on: what the compiler gave is checked when it is built, not at a user's call."""
+    good = [("_ZN3kvx16attn_tile_kernelIa", 96), ("_ZN3kvx17attn_split_kernelIa", 120), ("_ZN3kvx16attn_tile_kernelIb", 96)]
+    _build.check_registers(_ptxas(*good))
+    for bad in (good[1:2], [], good[:2] + [("_ZN3kvx16attn_tile_kernelIb", 88)], [("_ZN3kvx16attn_tile_kernelIb", 104)] + good):
+        with pytest.raises(RuntimeError, match="96 registers"):
+            _build.check_registers(_ptxas(*bad))
