@@ -11,8 +11,16 @@
 
 namespace kvx {
 
+// Splits of the key axis. Figures: us a call, bf16, 32 heads on 8 of 128 unless stated, `a x b` = a sequences of b keys.
+// CTAs of the split kernel to aim for, in fills of the GPU (more: an even end; fewer: less to join). 1 / 2 / 4 / 8: 4 x 50000
+// 150/146/147/149; 16 x 6000 86/85/88/90; 100 x 3000 205/205/205/215; 4-bit 8 x 8000 31/34/34/34, 100 x 3000 96/96/95/108.
 constexpr int kWaves = 4;
+// Keys of a split, at least. 128 / 256 / 512 / 1024 / 2048: 2 x 700 12/14/16/16/16; 8 x 1500 27/25/21/27/27; 16 x 6000
+// 88/88/88/94/86; 4-bit 2 x 700 11/12/13/13/13, 4 x 1500 14/14/14/19/19, 8 x 8000 40/39/34/31/33.
 constexpr int kMinKeys = 512;
+// Key tiles (of 128) of a split of the tile kernel, at least. 1 / 2 / 4 / 8: 64 tokens on 7936 keys 33/33/35/43, 2 x 40 tokens
+// on 2960 31/31/32/40, 32 on 968 22/25/27/31; 4-bit 64 on 7936 38/37/39/47.
+constexpr int kMinTiles = 4;
 // Rows of a sequence and kv head (tokens x group heads) up to which the split kernel is taken. Split against tile
 // kernel, us, bf16, 8 kv heads of 128: 16-bit cache, 32 sequences of 2000 keys: 12 rows 83/79, 16 rows 87/79,
 // 24 rows 99/77; 256 of 600: 151/168, 157/167, 189/169; 4 of 30000: 114/120, 118/118, 130/118. 4-bit cache: 16 rows
@@ -30,11 +38,6 @@ struct AttnPlan {
     int min_tiles;      // key tiles of a split, at least
     uint64_t workspace;
 };
-
-static bool power_of_two(float x) {
-    int e;
-    return std::isfinite(x) && x > 0.f && std::frexp(x, &e) == 0.5f && e >= -63 && e <= 64;
-}
 
 static int check_args(const kvx_attention* a) {
     if (a == nullptr) return fail(KVX_EINVAL, "args is NULL");
@@ -89,21 +92,12 @@ static AttnPlan plan_of(const kvx_attention* a, int sms) {
         pl.tile_tokens = (avg * group <= kTileRows / 2 ? kTileRows / 2 : kTileRows) / group;
         keys_per_tile = 128;
         fill = sms;
-        pl.min_tiles = 4;
+        pl.min_tiles = kMinTiles;
     } else {
-        // The row tiles of an item: the choice that reads the keys for the least work, a pass over them costing
-        // about as much as three row tiles (the widening and the loads).
-        int64_t least = INT64_MAX;
-        for (int nt = 1; nt <= 3; ++nt) {
-            if (8 * nt < group) continue;
-            const int per = a->cu_seqlens_q ? 8 * nt / group : 1;
-            const int64_t cost = (avg + per - 1) / per * (3 + nt);
-            if (cost < least) {
-                least = cost;
-                pl.nt = nt;
-                pl.tile_tokens = per;
-            }
-        }
+        // One pass over the keys for a sequence of average length. (A pass costs what it reads and widens, and a row tile less
+        // than that: two passes of fewer rows never pay.)
+        pl.nt = static_cast<int>((avg * group + 7) / 8);
+        pl.tile_tokens = a->cu_seqlens_q ? 8 * pl.nt / group : 1;
         const bool q4 = a->cache_bits == 4;
         keys_per_tile = q4 && pl.nt < 3 ? 128 : 64;
         fill = sms * (q4 && pl.nt == 1 ? 4 : 2) * kWaves;

@@ -167,6 +167,12 @@ __device__ __forceinline__ int block_of(const AttnParams& p, int j) {
     return p.block_shift >= 0 ? j >> p.block_shift : j / p.block_size;
 }
 
+// 16 bytes into shared memory, zeros unless `take`.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
+    const int n = take ? 16 : 0;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+
 // ---------------------------------------------------------------------------
 // Numbers
 // ---------------------------------------------------------------------------

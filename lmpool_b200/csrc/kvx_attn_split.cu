@@ -40,10 +40,6 @@ constexpr int kSplitWarps = 4;
 constexpr int kQ4Slices = 2;
 constexpr int kQ4Stages = 2;
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
-    const int n = take ? 16 : 0;
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {

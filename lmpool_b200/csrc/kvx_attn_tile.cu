@@ -201,10 +201,6 @@ __host__ __device__ constexpr uint32_t instruction(bool bf16, bool mn_major_b, i
            (static_cast<uint32_t>(n / 8) << 17) | (static_cast<uint32_t>(128 / 16) << 24);
 }
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool take) {
-    const int n = take ? 16 : 0;
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
 __device__ __forceinline__ void st_shared16(uint32_t dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -873,7 +869,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                         for (int s = 0; s < 32; s += kRowsPerStep) {
                             const int r = s + lane / kChunks, c = lane % kChunks;
                             const int64_t from = __shfl_sync(~0u, mine, r);
-                            cp16(chunk_at(base + h * C::kTileBytes, 32 * w + r, c), p.q + 16 * c + (from >= 0 ? from : 0), from >= 0);
+                            cp_async16(chunk_at(base + h * C::kTileBytes, 32 * w + r, c), p.q + 16 * c + (from >= 0 ? from : 0), from >= 0);
                         }
                     }
                     asm volatile("cp.async.wait_all;" ::: "memory");
@@ -936,7 +932,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
                         for (int s = 0; s < 32; s += kRowsPerStep) {
                             const int r = s + lane / kChunks, c = lane % kChunks;
                             const int64_t a = __shfl_sync(~0u, off, r);
-                            cp16(chunk_at(tile, 32 * w + r, c), plane + (a < 0 ? 0 : a) + 16 * c, a >= 0);
+                            cp_async16(chunk_at(tile, 32 * w + r, c), plane + (a < 0 ? 0 : a) + 16 * c, a >= 0);
                         }
                         asm volatile("cp.async.wait_all;" ::: "memory");
                         fence_async_shared();

@@ -4,6 +4,8 @@
 
 #include <cuda_runtime.h>
 
+#include <cmath>
+
 #include "kvx.h"
 
 namespace kvx {
@@ -13,6 +15,12 @@ constexpr int kMaxDevices = 64;
 int fail(int code, const char* fmt, ...);
 int cuda_fail(cudaError_t e, const char* what);
 int sm_count(int dev, int* out);
+
+// Whether x is a power of two in [2^-64, 2^63].
+inline bool power_of_two(float x) {
+    int e;
+    return std::isfinite(x) && x > 0.f && std::frexp(x, &e) == 0.5f && e >= -63 && e <= 64;
+}
 
 #define KVX_CUDA(call, what)                         \
     do {                                             \

@@ -15,7 +15,6 @@
 // bits, so x / s is at least 2^-12 (relative) away from t and stays on its side.
 
 #include <climits>
-#include <cmath>
 
 #include "kvx.h"
 #include "kvx_attn.cuh"
@@ -165,11 +164,6 @@ __global__ void __launch_bounds__(kQ4Threads) load_q4_kernel(const __grid_consta
     uint4* d = reinterpret_cast<uint4*>(dst + group * 32);
     d[0] = make_uint4(out[0], out[1], out[2], out[3]);
     d[1] = make_uint4(out[4], out[5], out[6], out[7]);
-}
-
-static bool power_of_two(float x) {
-    int e;
-    return std::isfinite(x) && x > 0.f && std::frexp(x, &e) == 0.5f && e >= -63 && e <= 64;
 }
 
 static int q4_launch(bool store, int32_t device, int32_t dtype, const void* key, const void* value,
