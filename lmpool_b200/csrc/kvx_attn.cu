@@ -22,9 +22,9 @@ constexpr int kMinKeys = 512;
 // on 2960 31/31/32/40, 32 on 968 22/25/27/31; 4-bit 64 on 7936 38/37/39/47.
 constexpr int kMinTiles = 4;
 // Rows of a sequence and kv head (tokens x group heads) up to which the split kernel is taken. Split against tile
-// kernel, us, bf16, 8 kv heads of 128: 16-bit cache, 32 sequences of 2000 keys: 12 rows 83/79, 16 rows 87/79,
-// 24 rows 99/77; 256 of 600: 151/168, 157/167, 189/169; 4 of 30000: 114/120, 118/118, 130/118. 4-bit cache: 16 rows
-// 69/99, 24 rows 91/99, 32 rows 122/99; 133/167, 177/232, 241/232; 83/157, 110/157, 146/161.
+// kernel, us, bf16, 8 kv heads of 128, 12, 16 and 24 rows. 16-bit cache, 32 sequences of 2000 keys: 82/90, 85/90, 97/90; 256 of
+// 600: 149/182, 154/182, 184/182; 4 of 30000: 116/157, 118/157, 130/157. 4-bit cache: 63/89, 67/89, 87/89; 121/207, 129/208,
+// 172/207; 81/151, 83/151, 108/151 (at 32 rows, in two passes of the split kernel: 122/99; 241/232; 146/161).
 constexpr int kFewRows16 = 16;
 constexpr int kFewRows4 = 24;
 constexpr int kTileRows = 256;          // rows of an item of the tile kernel

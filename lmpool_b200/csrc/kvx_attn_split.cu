@@ -15,14 +15,15 @@
 // 4-bit cache: the ring holds raw slices (16 keys: 1 KiB of codes and 128 bytes of scales of K
 // and of V at head_dim 128, each contiguous in a page), which lanes widen to fp16 and scale on
 // their way into the products, exactly. The fragments' order along head_dim and along the keys
-// is free as long as both operands agree, so a lane takes the codes that lie together: the
-// conversions, four instructions for eight elements with the scaling, bound this path, not
+// is free as long as both operands agree, so a lane takes the codes that lie together. A slice takes a warp about 450
+// instructions, half of them the widening (eight for eight elements with the scaling, and V's masks and shifts); with four warps a
+// scheduler the issue slots are 60 % busy and the ALU 51 %: half of what bounds this path is the latency between them, not
 // the bytes. Queries go to fp16 too, each row first divided by the power of two below its
 // largest element.
-// Measured, bf16, head_dim 128: 4 sequences of 40000 to 65610 keys, 4 rows of 8 kv heads: 139 to 143 us, 6.1 TB/s, 0.93
-// of the copy rate; 256 of 500 to 4095 keys, window 1024, 8 rows: 176 to 184 us, 0.89. 4-bit: 64 sequences of 1000 to 8191 keys, 4 rows:
-// 98 us, 0.53 of the copy rate; one of 131070 keys, 8 rows: 48 us, 0.48 (about 400 instructions of a warp per 16 keys, half of them
-// the widening). A call of a few sequences takes 11 us, of which the launch and the host's call are most.
+// Measured, bf16, head_dim 128: 4 sequences of 40000 to 65610 keys, 4 rows of 8 kv heads: 139 us, 6.1 TB/s, 0.95
+// of the copy rate; 256 of 500 to 4095 keys, window 1024, 8 rows: 174 us, 0.92. 4-bit: 64 sequences of 1000 to 8191 keys,
+// 4 rows: 97 us, 0.53 of the copy rate; one of 131070 keys, 8 rows: 48 us, 0.48. A call of a few sequences takes
+// 11 us, of which the launch and the host's call are most.
 // Weights: for a bf16 cache they are split in two bf16 numbers (2^-17 relative;
 // the tensor cores have time to spare here), for fp16 and 4-bit rounded to fp16, 2^7 higher (kLift).
 

@@ -40,11 +40,12 @@
 // 1/2, on the FMA units, with a degree-4 polynomial (relative error 2.8e-6, from a
 // weighted least-squares fit of 2^f; the weights are rounded to 2^-8 or 2^-11).
 //
-// Measured: a prompt of 8191 tokens, window 1024, 32 query heads on 8: 205 us (76 us of products at the rate of a large
-// library product); 4 prompts of 129 to 4095 tokens on up to 2001 earlier ones: 441 us (218 us); two of 3001 to 4096 on a
-// 4-bit cache: 391 us (183 us). A key tile takes two row tiles about 4200 clocks, of which the tensor cores are busy 2560:
-// the rest is issue slots, which the exponentials of 8 warps and the issuing of products share (more code or state
-// in either loop costs at once: two more values kept in the softmax loop, 4 %).
+// Measured: a prompt of 8191 tokens, window 1024, 32 query heads on 8: 201 us (76 us of products at the rate of a large
+// library product); 4 prompts of 129 to 4095 tokens on up to 2001 earlier ones: 438 us (218 us); two of 3001 to 4096 on a
+// 4-bit cache: 380 us (183 us). Counters of a prompt of 4096 tokens: tensor cores 48 % of the time busy, issue slots 51 %, ALU
+// 34 %, special-function units 30 %, no unit full; warps wait (most for tensor memory and barriers): what bounds it is the chain of
+// a step, scores to softmax to weights to product, of which two row tiles run at a time. Instructions in the softmax loop stand
+// in that chain: two more values kept in it, 4 %.
 //
 // Every wait is bounded: where one runs out, the CTA flags KVX_DEV_PIPE_TIMEOUT,
 // all warps leave their loops, and tensor memory is freed.
@@ -66,8 +67,8 @@ constexpr int kTileThreads = 640;
 constexpr int kTileKeys = 128;
 constexpr int kStepKeys = 64;                  // keys of a step
 constexpr int kHalfRows = 128;                 // rows of one of the two row tiles
-// Of 8 pairs of exponentials, on the FMA units: 3 on a 16-bit cache (8 prompts of 2048: 315 us, 338 with none), 1
-// on a 4-bit one, where the widening wants the issue slots (prompts on a 4-bit cache: 401 us, 422 with 3).
+// Of 8 pairs of exponentials, on the FMA units: 3 on a 16-bit cache (8 prompts of 2048: 319 us, 322 with none), 1
+// on a 4-bit one, where the widening wants the issue slots (two prompts on a 4-bit cache: 389 us, 407 with 3).
 template <bool Q4>
 constexpr int kFmaPairs = Q4 ? 1 : 3;
 constexpr float kFarScore = 1 << 20;           // log2 of a weight's factor is off by at most 2^-4 below this
@@ -486,9 +487,8 @@ __device__ __forceinline__ void issue_copies(const AttnParams& p, const TileMaps
         const int n = kt.end - kt.begin;
         const int last = it.pos0 + it.tokens - 1;
         const int32_t* table = p.table + it.seq * p.table_stride;
-        // This lane's page of a tile, if some row sees its keys. On a 4-bit cache it is read while the tile before is
-        // copied (five drafted tokens of 32 sequences, window 2048: 102 us, 109 without); a 16-bit ring has more in
-        // flight and gains nothing by it (256 sequences of 600 keys: 168 us, 176 with).
+        // This lane's page of a tile, if some row sees its keys. (Read a tile ahead it gains nothing: five drafted tokens
+        // of 32 sequences on a 4-bit cache, window 2048, 98 us, 97 so; prompts 389 and 385.)
         bool wanted = false;
         int id = -1, slot = 0;
         auto look_up = [&](int tile) {
@@ -501,7 +501,6 @@ __device__ __forceinline__ void issue_copies(const AttnParams& p, const TileMaps
                 if (blk < p.table_width) id = table[blk];
             }
         };
-        if (Q4) look_up(0);
         for (int op = 0; op < 2 * n; ++op, ring.next()) {
             if constexpr (!Q4) {
                 if (!warp_wait(&bars->empty[ring.at], ring.phase ^ 1, abort, p.status)) return;
@@ -511,8 +510,10 @@ __device__ __forceinline__ void issue_copies(const AttnParams& p, const TileMaps
                 }
                 if (!(op & 1)) look_up(op >> 1);
             }
-            if constexpr (Q4)
+            if constexpr (Q4) {
+                if (!(op & 1)) look_up(op >> 1);
                 if (!warp_wait(&bars->raw_empty[ring.at], ring.phase ^ 1, abort, p.status)) return;
+            }
             if (wanted && (id < 0 || id >= p.num_blocks)) {
                 atomicOr(p.status, KVX_DEV_BAD_SRC_ID);
                 id = -1;
@@ -544,7 +545,6 @@ __device__ __forceinline__ void issue_copies(const AttnParams& p, const TileMaps
                              16 * (D / 16), bar);
                 }
             }
-            if (Q4 && (op & 1)) look_up((op >> 1) + 1);
         }
     }
 }

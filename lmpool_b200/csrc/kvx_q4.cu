@@ -1,10 +1,11 @@
 // Rows into and out of the 4-bit paged cache (format: include/kvx.h).
 //
 // Both kernels give a thread one group of 16 elements: 32 bytes on the 16-bit
-// side, 8 bytes of codes and one scale byte on the 4-bit side. Bound: HBM
+// side, 8 bytes of codes and one scale byte on the 4-bit side. Floor: HBM
 // bytes, 2 + 9/16 per element; at a decode step's 256 tokens a launch's latency.
 // Measured, 8 kv heads of 128, rows stored and loaded again, two calls: 16384 tokens 42 us, 4.1 TB/s, 0.62 of the
-// copy rate (a row of a head is 64 bytes of codes and 8 of scales in a page); 256 tokens 23 us, the host's two calls.
+// copy rate (issue slots 80 % busy in the store, 68 % in the load: the conversion's instructions come first, then the
+// pieces: a row of a head is 64 bytes of codes and 8 of scales in a page); 256 tokens 23 us, the host's two calls.
 //
 // The codes are those of exact arithmetic. amax / 6 is divided in IEEE fp32: an
 // exact tie between two e4m3 values divides exactly, and a 16-bit amax that is no
