@@ -465,10 +465,12 @@ def paged_attention(
 
     Without ``cu_seqlens_q`` each sequence has one new token (``T == S``, decode). With it (int32 ``[S + 1]``, rising
     from 0) sequence ``s`` has the tokens ``cu_seqlens_q[s]`` to ``cu_seqlens_q[s + 1]``, the last of its context:
-    prompts, chunks of prompts, drafted tokens. Token at position ``p`` sees key ``j <= p`` if ``window`` is None, if
+    prompts, chunks of prompts, drafted tokens. (They may be mixed, but a call is planned for the average of new tokens a
+    sequence: single tokens and long prompts are quicker as two calls.) Token at position ``p`` sees key ``j <= p`` if ``window`` is None, if
     ``p - j < window`` or if ``j < sinks``. A token that sees no key gets zeros. Rows behind the last sequence are left
     as they were. ``out`` takes the result and must not overlap the inputs. ``scale`` (default ``D ** -0.5``) must be
-    positive. No gradient is recorded: this reads a serving cache.
+    positive. No gradient is recorded: this reads a serving cache. A value that is infinite or NaN decides its element of
+    the tokens that see it and reaches no other.
 
     Runs on the current stream without synchronising; lengths and tables are read on the device, so a captured call
     can be replayed with others. Bad page ids (their keys read as zeros) and lengths are recorded in the device's
