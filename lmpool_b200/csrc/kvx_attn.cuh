@@ -36,7 +36,7 @@ struct AttnParams {
     const int32_t* cu;                        // nullptr: one token per sequence
     int32_t* status;
     float* ws_o;                              // [tokens * heads][splits][D], not yet divided by the sum
-    float* ws_ml;                             // [tokens * heads][splits][2]: maximum of scale_log2 * score, sum
+    float* ws_ml;                             // [tokens * heads][splits][2]: what weights are relative to (scale_log2 * score), sum
     float scale_log2;                         // scale * log2(e) (* k_scale of a 4-bit cache)
     float out_scale;                          // v_scale of a 4-bit cache, else 1
     int32_t table_width, block_size, block_shift;   // block_shift < 0: not a power of two
@@ -417,12 +417,12 @@ __device__ __noinline__ void mend_row(const AttnParams& p, const AttnItem& it, c
     }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
-    // A partial result is in units of the maximum that the row's others are joined with.
+    // A partial result is relative to what the split's other elements are.
     const float mine = m == -INFINITY ? 0.f : m;
     float factor = sum > 0.f ? p.out_scale / sum : 0.f;
     if (p.splits > 1) {
         const float ref = p.ws_ml[at * 2];
-        factor = exp2f(mine - (ref == -INFINITY ? 0.f : ref) + kLift<typename std::conditional<Q4, __half, T>::type>);
+        factor = exp2f(mine - (ref == -INFINITY ? 0.f : ref));
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {

@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, Q4 && NT == 1 ? 4 : 2) attn_
     }
 
     float o[KS][NT][4];
-    float mx[NT][2], sum[NT][2];      // maxima in units of scale_log2 * score
+    float mx[NT][2], sum[NT][2];      // what weights are taken relative to: maxima of scale_log2 * score, less kLift
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         mx[nt][0] = mx[nt][1] = -INFINITY;
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, Q4 && NT == 1 ? 4 : 2) attn_
                 top[nt][c] = fmaxf(top[nt][c], __shfl_xor_sync(~0u, top[nt][c], 4));
                 top[nt][c] = fmaxf(top[nt][c], __shfl_xor_sync(~0u, top[nt][c], 8));
                 top[nt][c] = fmaxf(top[nt][c], __shfl_xor_sync(~0u, top[nt][c], 16));
-                grow |= top[nt][c] > mx[nt][c] + 8.f;              // also from no key to a first one
+                grow |= top[nt][c] - mx[nt][c] > 8.f + kLift<M>;   // also from no key to a first one
             }
         // Rescale only when a row's maximum grows by more than 2^8: until then weights stay below that (2^15 with kLift).
         if (__any_sync(~0u, grow)) {
@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, Q4 && NT == 1 ? 4 : 2) attn_
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    const float next = fmaxf(mx[nt][c], top[nt][c]);
+                    const float next = fmaxf(mx[nt][c], top[nt][c] - kLift<M>);
                     const float shrink = exp2_approx(mx[nt][c] - (next == -INFINITY ? 0.f : next));
                     mx[nt][c] = next;
                     sum[nt][c] *= shrink;
@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, Q4 && NT == 1 ? 4 : 2) attn_
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const float base = (mx[nt][c] == -INFINITY ? 0.f : mx[nt][c]) - kLift<M>;
+                const float base = mx[nt][c] == -INFINITY ? 0.f : mx[nt][c];
 #pragma unroll
                 for (int z = 0; z < NS; ++z) {
                     s[z][nt][c] = exp2_approx(s[z][nt][c] - base);

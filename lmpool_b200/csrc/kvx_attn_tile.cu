@@ -1134,7 +1134,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const __grid
             if (live && p.splits > 1) {
                 const int64_t at =
                     (static_cast<int64_t>(it.q0 + token) * p.heads + it.head * p.group + head) * p.splits + it.split;
-                *reinterpret_cast<float2*>(p.ws_ml + at * 2) = make_float2(top == -INFINITY ? top : top * scale, sum);
+                *reinterpret_cast<float2*>(p.ws_ml + at * 2) = make_float2(top == -INFINITY ? top : top * scale - kLift<M>, sum);
             }
             // The row's sum goes to warps 16-19 when they are done with the item before.
             if (!warp_wait(&bars->o_free[i], free_phase, abort, p.status)) break;

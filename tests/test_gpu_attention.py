@@ -872,6 +872,32 @@ def test_a_single_token_or_head_may_have_any_stride(require_gpu, q4):
     assert int(caches[0].sum()) > 0 and torch.equal(caches[0], caches[2]) and torch.equal(caches[1], caches[3])
 
 
+@pytest.mark.parametrize("dtype,q4", TYPES, ids=IDS)
+@pytest.mark.parametrize("tokens", [1, 3, 40], ids=["decode", "draft", "chunk"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_late_key_eight_binades_above_a_large_score(require_gpu, dtype, q4, tokens, dim):
+    """The largest weight that a maximum is not renewed for, at scores whose neighbours are 4 to 8 apart: 2^8 times the
+    first key's, still finite in the products. Scores are exact here (in units of log2, with scale = ln 2)."""
+    n, page = 200, 16
+    case = Case([n], 4, 1, dim, page, dtype, q4, q_lens=[tokens], seed=30)
+    high = 1536.0 if q4 else 2.0 ** 13
+    k, v = torch.zeros(n, 1, dim), torch.zeros(n, 1, dim)
+    k[0, 0, 0] = k[128, 0, 0] = high
+    k[128, 0, 16], k[128, 0, 17] = 8.0, 12.0                        # 12 gives the group the scale 2; no query reads it
+    v[0], v[128] = 6.0, 3.0
+    slots = case.tables[0].long()[torch.arange(n) // page] * page + torch.arange(n) % page
+    (at.store_kvcache_q4 if q4 else at.store_kvcache)(k.to(dtype).to(DEV), v.to(dtype).to(DEV), case.k, case.v, slots.to(DEV), page)
+    case.q = torch.zeros_like(case.q)
+    case.q[:, :, 0] = 2.0 ** 13 if not q4 else 2.0 ** 16 if dtype == torch.bfloat16 else 2.0 ** 15
+    case.q[:, :, 16] = 1.0
+    got = case.call(scale=math.log(2)).cpu().double()
+    kt.check_device_status(0)
+    want = (6.0 + 256 * 3.0) / 257
+    # half a step of the output, of each weight and, twice, the exponentials' 2^-18
+    step = HALF_STEP[dtype] + (2.0 ** -11 if q4 else HALF_STEP[dtype]) + 2.0 ** -17
+    assert ((got - want).abs() <= step * want).all()
+
+
 # ----------------------------------------------------------------------------------------------
 # Refusals
 # ----------------------------------------------------------------------------------------------
