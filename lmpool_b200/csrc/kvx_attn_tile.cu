@@ -487,8 +487,9 @@ __device__ __forceinline__ void issue_copies(const AttnParams& p, const TileMaps
         const int n = kt.end - kt.begin;
         const int last = it.pos0 + it.tokens - 1;
         const int32_t* table = p.table + it.seq * p.table_stride;
-        // This lane's page of a tile, if some row sees its keys. (Read a tile ahead it gains nothing: five drafted tokens
-        // of 32 sequences on a 4-bit cache, window 2048, 98 us, 97 so; prompts 389 and 385.)
+        // This lane's page of a tile, if some row sees its keys. On a 4-bit cache it is read while the tile before is copied
+        // (8 prompts of 2048, fp16: 363 us, 384 if read before the wait for its place in the ring, 371 after it; bf16: 389, 385
+        // and 394).
         bool wanted = false;
         int id = -1, slot = 0;
         auto look_up = [&](int tile) {
@@ -501,6 +502,7 @@ __device__ __forceinline__ void issue_copies(const AttnParams& p, const TileMaps
                 if (blk < p.table_width) id = table[blk];
             }
         };
+        if (Q4) look_up(0);
         for (int op = 0; op < 2 * n; ++op, ring.next()) {
             if constexpr (!Q4) {
                 if (!warp_wait(&bars->empty[ring.at], ring.phase ^ 1, abort, p.status)) return;
@@ -510,10 +512,8 @@ __device__ __forceinline__ void issue_copies(const AttnParams& p, const TileMaps
                 }
                 if (!(op & 1)) look_up(op >> 1);
             }
-            if constexpr (Q4) {
-                if (!(op & 1)) look_up(op >> 1);
+            if constexpr (Q4)
                 if (!warp_wait(&bars->raw_empty[ring.at], ring.phase ^ 1, abort, p.status)) return;
-            }
             if (wanted && (id < 0 || id >= p.num_blocks)) {
                 atomicOr(p.status, KVX_DEV_BAD_SRC_ID);
                 id = -1;
@@ -545,6 +545,7 @@ __device__ __forceinline__ void issue_copies(const AttnParams& p, const TileMaps
                              16 * (D / 16), bar);
                 }
             }
+            if (Q4 && (op & 1)) look_up((op >> 1) + 1);
         }
     }
 }
